@@ -396,6 +396,63 @@ size_t k3gpu_lm_head_argmax_workspace(int T, int in, int vocab);
 int k3gpu_lm_head_argmax(int *arg, const float *X, int ldx, const uint16_t *W, int in, int vocab, int T,
                          void *workspace, size_t ws_bytes, void *stream);
 
+/* ------------------------------------------------------- fitting a draft head ---- */
+/* The K largest logits of each row (argmax_'s order, src/cli/k3_run.c:138-139, carried on):
+ * val [rows][K] descending and idx [rows][K] their ids, equal values by ascending id; NaN
+ * is never taken; a row with fewer than K values that are not NaN ends in idx -1, val
+ * -inf. logits [rows][vocab], e.g. a verify sweep's (k3gpu_model_verify): the teacher
+ * entries of k3gpu_lm_head_distill. 1 <= K <= 128, rows <= 65535. The workspace is 16-byte
+ * aligned. */
+size_t k3gpu_topk_logits_workspace(int rows, int vocab, int K);
+int k3gpu_topk_logits(int *idx, float *val, const float *logits, int rows, int vocab, int K,
+                      void *workspace, size_t ws_bytes, void *stream);
+
+/* The losses of a draft head over the lm_head product (k3gpu_lm_head_argmax's form: the
+ * [T][vocab] logits are never written). X [T][in] bf16 bits, row stride ldx elements (any
+ * ldx >= in; rows that are 16-byte aligned are read in place), W [vocab][in] bf16 bits,
+ * 16-byte aligned; z = X W^T with exact products and fp32 sums.
+ * Limits: in % 8 == 0, in <= 65536, vocab <= 2^24, T <= 2^20; the workspace is 256-byte
+ * aligned, the same for a loss and its gradient. The reference has no training code; these
+ * have no counterpart there.
+ *
+ * Softmax cross entropy: lse[t] = ln sum_v e^z[t][v], loss[t] = lse[t] - z[t][label[t]], fp32
+ * [T]. A negative label is a row without a target: its loss, lse and gradient are 0, and
+ * nothing of its hidden state is read. A label >= vocab is treated so and flagged (device
+ * status bit 1). */
+size_t k3gpu_lm_head_xent_workspace(int T, int in, int vocab);
+int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, int ldx, const uint16_t *W,
+                       const int *label, int in, int vocab, int T, void *workspace,
+                       size_t ws_bytes, void *stream);
+/* Its gradient, from the lse that k3gpu_lm_head_xent gave for the same X, W and labels:
+ *   dz[t][v] = g[t] (e^(z[t][v] - lse[t]) - [v == label[t]]),  dX = dz W,  dW = dz^T X
+ * with g [T] the loss's incoming gradient (NULL: 1). dX [T][in] (row stride lddx) and dW
+ * [vocab][in] (16-byte aligned) are bf16 bits, written whole, not added to; either may be
+ * NULL (a frozen head needs no dW). dz is rounded to bf16 once; the sums are fp32. The
+ * vocabulary is taken in pieces, so the workspace does not grow with T * vocab. Neither output
+ * may overlap an input. */
+int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, const float *g,
+                            const float *lse, const uint16_t *X, int ldx, const uint16_t *W,
+                            const int *label, int in, int vocab, int T, void *workspace,
+                            size_t ws_bytes, void *stream);
+/* Distillation from a teacher's top logits: ids, top [T][K] the teacher's entries of each row
+ * (k3gpu_topk_logits of its logits), in any order; temp > 0 divides both sides' logits.
+ *   q = softmax(top[t] / temp) over the row's entries,  lse[t] = ln sum_v e^(z[t][v] / temp)
+ *   loss[t] = sum_k q_k (ln q_k - z[t][id_k] / temp + lse[t])      (KL of q from the head)
+ * An entry with a negative id or a logit of -inf is empty; one with id >= vocab too, and it is
+ * flagged. An id may occur twice: the masses add. A row without entries has loss, lse and
+ * gradient 0 and its hidden state is not read. A NaN or +inf teacher logit makes its row's
+ * loss NaN. 1 <= K <= 128. */
+size_t k3gpu_lm_head_distill_workspace(int T, int in, int vocab, int K);
+int k3gpu_lm_head_distill(float *loss, float *lse, const uint16_t *X, int ldx, const uint16_t *W,
+                          const int *ids, const float *top, int K, float temp, int in, int vocab,
+                          int T, void *workspace, size_t ws_bytes, void *stream);
+/* Its gradient (arguments as k3gpu_lm_head_xent_grad):
+ *   dz[t][v] = g[t] / temp (e^(z[t][v] / temp - lse[t]) - sum_{k: id_k = v} q_k) */
+int k3gpu_lm_head_distill_grad(uint16_t *dX, int lddx, uint16_t *dW, const float *g,
+                               const float *lse, const uint16_t *X, int ldx, const uint16_t *W,
+                               const int *ids, const float *top, int K, float temp, int in,
+                               int vocab, int T, void *workspace, size_t ws_bytes, void *stream);
+
 /* ------------------------------------------------------- norms and AttnRes ------ */
 /* k3_rmsnorm (src/core/k3_ops.c:132-140) over T rows: x, y [T][n] (y may be x), w [n];
  * double sum of squares, 1/sqrt(ss/n + eps) rounded to float, y = (w * x) * inv. */

@@ -205,6 +205,14 @@ _SIGS = {
     "k3gpu_matmul_bf16_batch": ([VP, I, VP, I, VP, I, I, I, VP, SZ, VP], I),
     "k3gpu_lm_head_argmax_workspace": ([I, I, I], SZ),
     "k3gpu_lm_head_argmax": ([VP, VP, I, VP, I, I, I, VP, SZ, VP], I),
+    "k3gpu_topk_logits_workspace": ([I, I, I], SZ),
+    "k3gpu_topk_logits": ([VP, VP, VP, I, I, I, VP, SZ, VP], I),
+    "k3gpu_lm_head_xent_workspace": ([I, I, I], SZ),
+    "k3gpu_lm_head_xent": ([VP, VP, VP, I, VP, VP, I, I, I, VP, SZ, VP], I),
+    "k3gpu_lm_head_xent_grad": ([VP, I, VP, VP, VP, VP, I, VP, VP, I, I, I, VP, SZ, VP], I),
+    "k3gpu_lm_head_distill_workspace": ([I, I, I, I], SZ),
+    "k3gpu_lm_head_distill": ([VP, VP, VP, I, VP, VP, VP, I, F, I, I, I, VP, SZ, VP], I),
+    "k3gpu_lm_head_distill_grad": ([VP, I, VP, VP, VP, VP, I, VP, VP, VP, I, F, I, I, I, VP, SZ, VP], I),
     "k3gpu_attn_res": ([VP, VP, VP, VP, VP, I, I, I, F, VP], I),
     "k3gpu_moe_prefill_workspace": ([C.POINTER(K3GpuMoeCfg), I], SZ),
     "k3gpu_moe_prefill": ([VP, VP, VP, VP, C.POINTER(K3GpuMoeW), C.POINTER(K3GpuMoeCfg), I, VP, SZ, VP], I),
@@ -575,6 +583,133 @@ def lm_head_argmax(X, W, ws=None, stream=None):
     check(lib.k3gpu_lm_head_argmax(arg.data_ptr(), X.data_ptr(), X.stride(0), ptr(W), n_in, vocab, T, ptr(ws),
                                    ws.numel(), stream_ptr(stream)), "k3gpu_lm_head_argmax")
     return arg
+
+
+# ------------------------------------------------------- fitting a draft head ------
+def _on(device, *tensors):
+    """Every tensor (None skipped) on the one CUDA device."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise K3Error(f"expected every tensor on {device}, got one on {t.device}")
+
+
+def _head_args(X, W, ws, need):
+    """The checks the draft-head losses share; the workspace when the caller gave none."""
+    for name, t in (("X", X), ("W", W)):
+        if not t.is_cuda or t.dim() != 2 or t.element_size() != 2 or t.dtype == torch.float16:
+            raise K3Error(f"{name}: expected a 2-D CUDA tensor of bfloat16 (or its bits)")
+    if X.shape[1] != W.shape[1]:
+        raise K3Error(f"X {tuple(X.shape)} and W {tuple(W.shape)} differ in width")
+    if X.stride(1) != 1 or (X.shape[0] > 1 and X.stride(0) < X.shape[1]):
+        raise K3Error("X: expected rows of consecutive elements that do not overlap")
+    return ws if ws is not None else workspace(need, X.device)
+
+
+def _row_stride(X):
+    return X.stride(0) if X.shape[0] > 1 else X.shape[1]
+
+
+def _rows_of(name, t, shape, dtype):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise K3Error(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return ptr(t)
+
+
+def topk_logits(logits, K, ws=None, stream=None):
+    """The K largest logits of each row of logits [rows][vocab]: (ids int32, values fp32)
+    [rows][K], descending, equal values by ascending id, NaN never taken; a row that runs out
+    ends in id -1, -inf. The teacher entries of lm_head_distill."""
+    if logits.dim() != 2 or logits.dtype != torch.float32:
+        raise K3Error("logits: expected fp32 [rows][vocab]")
+    rows, vocab = logits.shape
+    with torch.cuda.device(logits.device):
+        idx = torch.empty((rows, K), dtype=torch.int32, device=logits.device)
+        val = torch.empty((rows, K), dtype=torch.float32, device=logits.device)
+        if rows == 0:
+            return idx, val
+        ws = ws if ws is not None else workspace(lib.k3gpu_topk_logits_workspace(rows, vocab, K), logits.device)
+        _on(logits.device, ws)
+        check(lib.k3gpu_topk_logits(ptr(idx), ptr(val), ptr(logits), rows, vocab, K, ptr(ws), ws.numel(),
+                                    stream_ptr(stream)), "k3gpu_topk_logits")
+    return idx, val
+
+
+def lm_head_xent(X, W, label, ws=None, stream=None):
+    """Softmax cross entropy of the lm_head product X [T][in] . W^T (bf16, the logits never
+    written) against label int32 [T]: (loss, lse) fp32 [T]. A negative label is a row without a
+    target: loss, lse and gradient 0."""
+    T, vocab = X.shape[0], W.shape[0]
+    with torch.cuda.device(X.device):
+        loss = torch.empty(T, dtype=torch.float32, device=X.device)
+        lse = torch.empty(T, dtype=torch.float32, device=X.device)
+        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_xent_workspace(T, X.shape[1], vocab))
+        _on(X.device, W, label, ws)
+        lab = _rows_of("label", label, (T,), torch.int32)
+        if T == 0:
+            return loss, lse
+        check(lib.k3gpu_lm_head_xent(ptr(loss), ptr(lse), X.data_ptr(), _row_stride(X), ptr(W), lab, X.shape[1], vocab, T,
+                                     ptr(ws), ws.numel(), stream_ptr(stream)), "k3gpu_lm_head_xent")
+    return loss, lse
+
+
+def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
+    """The gradient of lm_head_xent from its lse and the loss's incoming gradient g fp32 [T]
+    (None: 1): (dX [T][in], dW [vocab][in]) bf16, None where not needed (a frozen head)."""
+    T, vocab = X.shape[0], W.shape[0]
+    with torch.cuda.device(X.device):
+        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_xent_workspace(T, X.shape[1], vocab))
+        _on(X.device, W, label, lse, g, ws)
+        lab, ls = _rows_of("label", label, (T,), torch.int32), _rows_of("lse", lse, (T,), torch.float32)
+        gp = _rows_of("g", g, (T,), torch.float32) if g is not None else None
+        dX = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device) if need_dx else None
+        dW = torch.empty(W.shape, dtype=torch.bfloat16, device=X.device) if need_dw else None
+        if T == 0:
+            return dX, dW.zero_() if need_dw else None
+        if need_dx or need_dw:
+            check(lib.k3gpu_lm_head_xent_grad(ptr(dX), X.shape[1], ptr(dW), gp, ls, X.data_ptr(), _row_stride(X), ptr(W),
+                                              lab, X.shape[1], vocab, T, ptr(ws), ws.numel(), stream_ptr(stream)),
+                  "k3gpu_lm_head_xent_grad")
+    return dX, dW
+
+
+def lm_head_distill(X, W, ids, top, temp=1.0, ws=None, stream=None):
+    """KL of the teacher's top logits (ids int32, top fp32 [T][K], e.g. topk_logits of its
+    sweep) from the head's softmax, both at temperature temp: (loss, lse) fp32 [T]. Entries with a
+    negative id or a logit of -inf are empty; a row without entries has loss, lse and
+    gradient 0."""
+    T, vocab, K = X.shape[0], W.shape[0], ids.shape[1]
+    with torch.cuda.device(X.device):
+        loss = torch.empty(T, dtype=torch.float32, device=X.device)
+        lse = torch.empty(T, dtype=torch.float32, device=X.device)
+        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_distill_workspace(T, X.shape[1], vocab, K))
+        _on(X.device, W, ids, top, ws)
+        ip, tp = _rows_of("ids", ids, (T, K), torch.int32), _rows_of("top", top, (T, K), torch.float32)
+        if T == 0:
+            return loss, lse
+        check(lib.k3gpu_lm_head_distill(ptr(loss), ptr(lse), X.data_ptr(), _row_stride(X), ptr(W), ip, tp, K, float(temp),
+                                        X.shape[1], vocab, T, ptr(ws), ws.numel(), stream_ptr(stream)),
+              "k3gpu_lm_head_distill")
+    return loss, lse
+
+
+def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
+    """The gradient of lm_head_distill (arguments and results as lm_head_xent_grad)."""
+    T, vocab, K = X.shape[0], W.shape[0], ids.shape[1]
+    with torch.cuda.device(X.device):
+        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_distill_workspace(T, X.shape[1], vocab, K))
+        _on(X.device, W, ids, top, lse, g, ws)
+        ip, tp = _rows_of("ids", ids, (T, K), torch.int32), _rows_of("top", top, (T, K), torch.float32)
+        ls = _rows_of("lse", lse, (T,), torch.float32)
+        gp = _rows_of("g", g, (T,), torch.float32) if g is not None else None
+        dX = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device) if need_dx else None
+        dW = torch.empty(W.shape, dtype=torch.bfloat16, device=X.device) if need_dw else None
+        if T == 0:
+            return dX, dW.zero_() if need_dw else None
+        if need_dx or need_dw:
+            check(lib.k3gpu_lm_head_distill_grad(ptr(dX), X.shape[1], ptr(dW), gp, ls, X.data_ptr(), _row_stride(X),
+                                                 ptr(W), ip, tp, K, float(temp), X.shape[1], vocab, T, ptr(ws),
+                                                 ws.numel(), stream_ptr(stream)), "k3gpu_lm_head_distill_grad")
+    return dX, dW
 
 
 # ------------------------------------------------------------- decoder layer -------

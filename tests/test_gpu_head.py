@@ -1,0 +1,371 @@
+"""The draft-head losses (k3gpu_lm_head_xent, k3gpu_lm_head_distill and their gradients)
+against the formulas in 64 bits.
+
+Tolerances, element by element, from the arithmetic the header states. Products of bf16
+pairs are exact. A product's fp32 sum of n terms takes at most n additions, each off by at
+most 2^-23 of the partial sum, which sum |x w| =: S bounds; the tensor core adds 16 products
+a step, so ez = (n / 16 + 16) 2^-23 S bounds a logit's error. Then, with one temperature:
+  lse, loss   off by at most max ez (a softmax moves by no more than its logits do), twice for
+              the loss, plus 2^-21 of the magnitudes for the scaling by log2 e and the exp2
+  p           relative: 2 max ez + 2^-19 |z| (argument rounding of the exp2) + 2^-20
+  dz          |dz| 2^-8 (one bf16 rounding is at most 2^-9; doubled) + that times p
+  dX, dW      the sum of their terms' errors, the sums' own (n + 16) 2^-23 sum |.|, and the bf16
+              rounding of the output, 2^-8 of it (at most 2^-9)
+"""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+sys.path.insert(0, HERE)
+sys.path.insert(0, os.path.dirname(HERE))
+from k3lib import load  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def k3():
+    return load()
+
+
+def inputs(T, n, vocab, seed, spread=2.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    X = torch.randn((T, n), generator=gen, device="cuda").bfloat16()
+    W = (torch.randn((vocab, n), generator=gen, device="cuda") * (spread / math.sqrt(n))).bfloat16()
+    g = torch.rand(T, generator=gen, device="cuda") * 2 - 0.5
+    return X, W, g, gen
+
+
+def targets_xent(label, vocab):
+    """(ids, mass, entropy, live) of labels: one entry of mass 1."""
+    live = (label >= 0) & (label < vocab)
+    return label.long().clamp(0, vocab - 1)[:, None], live.double()[:, None], 0.0, live
+
+
+def targets_distill(ids, top, temp, vocab):
+    ok = (ids >= 0) & (ids < vocab) & (top != -math.inf)
+    live = ok.any(1)
+    t = torch.where(ok, top.double(), -math.inf)
+    t = (t - torch.where(live, t.amax(1), 0.0)[:, None]) / temp
+    e = torch.where(ok, t.exp(), 0.0)
+    s = e.sum(1, keepdim=True)
+    q = torch.where(live[:, None], e / s, 0.0)
+    ent = torch.where(q > 0, q * (t - s.log()), 0.0).sum(1)
+    return ids.long().clamp(0, vocab - 1), q, torch.where(live, ent, 0.0), live
+
+
+def formula(X, W, tgt, temp, g):
+    """Everything in 64 bits, and the bounds of the module's docstring."""
+    ids, q, ent, live = tgt
+    lv = live.double()
+    Xd = torch.where(live[:, None], X.double(), 0.0)
+    Wd = W.double()
+    n, vocab, T = X.shape[1], W.shape[0], X.shape[0]
+    z = (Xd @ Wd.T) / temp
+    S = (Xd.abs() @ Wd.abs().T) / temp
+    ez = (n / 16 + 16) * 2.0 ** -23 * S
+    ez1 = ez.amax(1)
+    lse = torch.logsumexp(z, 1)
+    zt = (q * z.gather(1, ids)).sum(1)
+    loss = (ent + lse - zt) * lv
+    mag = lse.abs() + z.abs().amax(1) + torch.as_tensor(ent, device=z.device).abs() + 1
+    b_lse = ez1 + 2.0 ** -21 * mag
+    b_loss = 2 * ez1 + 2.0 ** -21 * mag
+    p = (z - lse[:, None]).exp()
+    dz = p.clone().scatter_add_(1, ids, -q)
+    gt = (g.double() / temp * lv)[:, None]
+    dz *= gt
+    b_dz = dz.abs() * 2.0 ** -8 + gt.abs() * p * ((2 * ez1 + 2.0 ** -20)[:, None] + 2.0 ** -19 * (z.abs() + mag[:, None]))
+    b_dz += gt.abs() * torch.zeros_like(p).scatter_add_(1, ids, q) * 2.0 ** -22
+    dX, dW = dz @ Wd, dz.T @ Xd
+    b_dX = b_dz @ Wd.abs() + (vocab + 16) * 2.0 ** -23 * (dz.abs() @ Wd.abs()) + dX.abs() * 2.0 ** -8
+    b_dW = b_dz.T @ Xd.abs() + (T + 16) * 2.0 ** -23 * (dz.abs().T @ Xd.abs()) + dW.abs() * 2.0 ** -8
+    return {"loss": (loss, b_loss), "lse": (lse * lv, b_lse), "dX": (dX, b_dX), "dW": (dW, b_dW)}
+
+
+def holds(name, got, want):
+    value, bound = want
+    assert got.shape == value.shape
+    off = (got.double() - value).abs()
+    assert bool(torch.isfinite(got).all()), name
+    worst = float((off - bound).max())
+    assert worst <= 1e-30, (name, worst, float(off.max()))
+
+
+def xent_all(k3, X, W, label, g, **kw):
+    loss, lse = k3.lm_head_xent(X, W, label)
+    dX, dW = k3.lm_head_xent_grad(X, W, label, lse, g=g, **kw)
+    return {"loss": loss, "lse": lse, "dX": dX, "dW": dW}
+
+
+def distill_all(k3, X, W, ids, top, temp, g, **kw):
+    loss, lse = k3.lm_head_distill(X, W, ids, top, temp=temp)
+    dX, dW = k3.lm_head_distill_grad(X, W, ids, top, lse, temp=temp, g=g, **kw)
+    return {"loss": loss, "lse": lse, "dX": dX, "dW": dW}
+
+
+# one token, one id, one 16-byte row; edges of the tiles (128, 256, 64) on each side; several
+# pieces of the vocabulary (the last two)
+SIZES = [(1, 8, 1), (1, 64, 1000), (3, 72, 255), (129, 136, 257), (128, 64, 256), (257, 512, 1024), (300, 1000, 3001),
+         (40, 7168, 2000), (16389, 64, 5000), (8200, 200, 10007)]
+
+
+@pytest.mark.parametrize("T,n,vocab", SIZES)
+@pytest.mark.parametrize("masked", [0.0, 0.4])
+def test_xent(k3, T, n, vocab, masked):
+    X, W, g, gen = inputs(T, n, vocab, T * 7 + n + vocab)
+    label = torch.randint(0, vocab, (T,), generator=gen, device="cuda")
+    label = torch.where(torch.rand(T, generator=gen, device="cuda") < masked, -100, label).int()
+    got = xent_all(k3, X, W, label, g)
+    want = formula(X, W, targets_xent(label, vocab), 1.0, g)
+    for name in want:
+        holds(name, got[name], want[name])
+    assert k3.device_status(0) == 0
+
+
+@pytest.mark.parametrize("T,n,vocab,K,temp", [(1, 8, 1, 1, 1.0), (1, 64, 1000, 128, 2.0), (130, 136, 257, 7, 0.5),
+                                              (300, 1000, 3001, 64, 1.0), (257, 72, 5, 33, 1.5),
+                                              (8200, 200, 10007, 16, 3.0)])
+def test_distill(k3, T, n, vocab, K, temp):
+    """Entries in any order, doubled ids (vocab 5 has nothing else), empty entries, rows without any."""
+    X, W, g, gen = inputs(T, n, vocab, T + n + vocab + K)
+    ids = torch.randint(0, vocab, (T, K), generator=gen, device="cuda")
+    top = torch.randn((T, K), generator=gen, device="cuda") * 3 + 5
+    ids = torch.where(torch.rand((T, K), generator=gen, device="cuda") < 0.1, -1, ids)
+    if T > 2:
+        ids[T // 2] = -1
+        top[T // 3] = -math.inf
+    top[0, 0] = -math.inf if K > 1 else 0.25
+    ids = ids.int()
+    got = distill_all(k3, X, W, ids, top, temp, g)
+    want = formula(X, W, targets_distill(ids, top, temp, vocab), temp, g)
+    for name in want:
+        holds(name, got[name], want[name])
+    assert k3.device_status(0) == 0
+
+
+def test_distill_of_one_entry_is_xent(k3):
+    """K = 1 has mass 1 whatever its logit: the same numbers as the cross entropy."""
+    X, W, g, gen = inputs(70, 256, 900, 3)
+    label = torch.randint(-1, 900, (70,), generator=gen, device="cuda").int()
+    a = xent_all(k3, X, W, label, g)
+    top = torch.randn((70, 1), generator=gen, device="cuda") * 50
+    b = distill_all(k3, X, W, label[:, None].contiguous(), top, 1.0, g)
+    for name in a:
+        assert torch.equal(a[name], b[name]), name
+
+
+def test_teacher_of_lowest_values(k3):
+    """Teacher logits of the type's lowest value: alone they share the mass; beside a larger one
+    they get none of it, though their distance from it overflows at a low temperature."""
+    X, W, g, gen = inputs(2, 64, 100, 4)
+    low = torch.finfo(torch.float32).min
+    ids = torch.tensor([[3, 7, 11, 13], [3, 7, 11, 13]], dtype=torch.int32, device="cuda")
+    top = torch.tensor([[low] * 4, [low, 1.0, low, 2.0]], device="cuda")
+    got = distill_all(k3, X, W, ids, top, 0.25, g)
+    want = formula(X, W, targets_distill(ids, top, 0.25, 100), 0.25, g)
+    for name in want:
+        holds(name, got[name], want[name])
+
+
+@pytest.mark.parametrize("n", [0, 1])
+def test_rows_without_target(k3, n):
+    """None (or one) of the rows has a target: zeros, whatever NaN the others hold."""
+    X, W, g, gen = inputs(150, 128, 700, 5)
+    label = torch.full((150,), -1, dtype=torch.int32, device="cuda")
+    keep = torch.zeros(150, dtype=torch.bool, device="cuda")
+    if n:
+        label[77], keep[77] = 699, True
+    Xn = torch.where(keep[:, None], X, torch.full_like(X, float("nan")))
+    got = xent_all(k3, Xn, W, label, torch.where(keep, g, torch.full_like(g, float("nan"))))
+    want = formula(X, W, targets_xent(label, 700), 1.0, g)
+    for name in want:
+        holds(name, got[name], want[name])
+    for name in ("loss", "lse", "dX"):
+        assert (got[name][~keep] == 0).all()
+
+
+def test_out_of_range_targets_are_flagged_and_left_out(k3):
+    X, W, g, gen = inputs(20, 64, 300, 6)
+    label = torch.arange(20, dtype=torch.int32, device="cuda")
+    label[4], label[9] = 300, 2 ** 31 - 1
+    k3.device_status(0)
+    got = xent_all(k3, X, W, label, g)
+    assert k3.device_status(0) == 1
+    want = formula(X, W, targets_xent(label, 300), 1.0, g)
+    for name in want:
+        holds(name, got[name], want[name])
+    ids = torch.stack([label, torch.full_like(label, 7)], 1)
+    top = torch.ones((20, 2), device="cuda")
+    got = distill_all(k3, X, W, ids, top, 1.0, g)
+    assert k3.device_status(0) == 1
+    want = formula(X, W, targets_distill(ids, top, 1.0, 300), 1.0, g)
+    for name in want:
+        holds(name, got[name], want[name])
+
+
+def test_nan_stays_in_its_row(k3):
+    """A NaN hidden state or teacher logit of a row that counts: its loss and dX are NaN, the
+    other rows' are what they are without it."""
+    X, W, g, gen = inputs(33, 64, 600, 7)
+    label = torch.randint(0, 600, (33,), generator=gen, device="cuda").int()
+    clean = xent_all(k3, X, W, label, g)
+    X2 = X.clone()
+    X2[5, 3] = float("nan")
+    got = xent_all(k3, X2, W, label, g, need_dw=False)
+    other = torch.arange(33, device="cuda") != 5
+    for name in ("loss", "lse", "dX"):
+        assert torch.isnan(got[name][5]).all()
+        assert torch.equal(got[name][other], clean[name][other])
+    top = torch.randn((33, 4), generator=gen, device="cuda")
+    ids = torch.randint(0, 600, (33, 4), generator=gen, device="cuda").int()
+    clean = distill_all(k3, X, W, ids, top, 1.0, g)
+    for bad in (float("nan"), math.inf):
+        top2 = top.clone()
+        top2[8, 2] = bad
+        got = distill_all(k3, X, W, ids, top2, 1.0, g, need_dw=False)
+        assert torch.isnan(got["loss"][8])
+        other = torch.arange(33, device="cuda") != 8
+        for name in ("loss", "lse", "dX"):
+            assert torch.equal(got[name][other], clean[name][other])
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_strided_and_unaligned_hidden_states(k3, masked):
+    """X a slice of wider rows: at an aligned stride it is read in place, at an odd one it is
+    packed first; the numbers do not change. Nothing beside the slice is read."""
+    X, W, g, gen = inputs(140, 200, 400, 8)
+    label = torch.randint(0, 400, (140,), generator=gen, device="cuda").int()
+    if masked:
+        label[::3] = -1
+    base = xent_all(k3, X, W, label, g)
+    for width, off in ((208, 8), (211, 5), (203, 0)):
+        wide = torch.full((140, width), float("nan"), dtype=torch.bfloat16, device="cuda")
+        wide[:, off:off + 200] = X
+        got = xent_all(k3, wide[:, off:off + 200], W, label, g)
+        for name in base:
+            assert torch.equal(got[name], base[name]), (name, width, off)
+
+
+def test_strided_dx_leaves_its_neighbours(k3):
+    """dX into a slice of a wider buffer, aligned and not: only the slice is written."""
+    X, W, g, gen = inputs(140, 72, 300, 9)
+    label = torch.randint(-1, 300, (140,), generator=gen, device="cuda").int()
+    _, lse = k3.lm_head_xent(X, W, label)
+    want, _ = k3.lm_head_xent_grad(X, W, label, lse, g=g, need_dw=False)
+    lib = k3.lib
+    ws = k3.workspace(lib.k3gpu_lm_head_xent_workspace(140, 72, 300))
+    for width, off in ((80, 8), (77, 3)):
+        wide = torch.full((140, width), 7.0, dtype=torch.bfloat16, device="cuda")
+        part = wide[:, off:off + 72]
+        k3.check(lib.k3gpu_lm_head_xent_grad(part.data_ptr(), width, None, k3.ptr(g), k3.ptr(lse), k3.ptr(X), 72,
+                                             k3.ptr(W), k3.ptr(label), 72, 300, 140, k3.ptr(ws), ws.numel(),
+                                             k3.stream_ptr()))
+        assert torch.equal(part, want)
+        assert (wide[:, :off] == 7).all() and (wide[:, off + 72:] == 7).all()
+
+
+def test_gradient_against_differences(k3):
+    """Central differences of the loss itself: a step of d along a direction of X moves g . loss by
+    2 d <dX, direction>. X + d u is exact in bf16 (steps of 2^-3 on a grid), the third
+    derivative of a log-sum-exp of logits moved by |W u| is at most |W u|^3 / 6 a row, and the
+    losses carry their own bounds."""
+    T, n, vocab, d = 24, 64, 500, 2.0 ** -3
+    _, W, g, gen = inputs(T, n, vocab, 10, spread=0.5)
+    X = (torch.randint(-8, 9, (T, n), generator=gen, device="cuda") / 8).bfloat16()
+    u = torch.where(torch.rand((T, n), generator=gen, device="cuda") < 0.5, -1.0, 1.0).bfloat16()
+    label = torch.randint(0, vocab, (T,), generator=gen, device="cuda").int()
+    ids = torch.randint(0, vocab, (T, 5), generator=gen, device="cuda").int()
+    top = torch.randn((T, 5), generator=gen, device="cuda")
+    for fwd, bwd in ((lambda x: k3.lm_head_xent(x, W, label),
+                      lambda x, l: k3.lm_head_xent_grad(x, W, label, l, g=g)[0]),
+                     (lambda x: k3.lm_head_distill(x, W, ids, top),
+                      lambda x, l: k3.lm_head_distill_grad(x, W, ids, top, l, g=g)[0])):
+        _, lse = fwd(X)
+        dX = bwd(X, lse).double()
+        up, down = fwd(X + d * u)[0].double(), fwd(X - d * u)[0].double()
+        got = (up - down) * g.double() / (2 * d)
+        want = (dX * u.double()).sum(1)
+        move = (u.double() @ W.double().T).abs().amax(1) * 2            # of z_i - E z, at most
+        S = (X.double().abs() + d) @ W.double().abs().T
+        ez = (n / 16 + 16) * 2.0 ** -23 * S.amax(1)
+        loss_err = (2 * ez + 2.0 ** -21 * (up.abs() * 2 + 20)) / d
+        grad_err = 2.0 ** -7 * (W.double().abs().amax(1).max() * n * 2 + dX.abs().sum(1) / g.double().abs())
+        assert ((got - want).abs() <= g.double().abs() * (move ** 3 * d * d / 6 + loss_err + grad_err)).all()
+
+
+def test_frozen_head_and_head_alone(k3):
+    X, W, g, gen = inputs(100, 264, 777, 11)
+    label = torch.randint(-1, 777, (100,), generator=gen, device="cuda").int()
+    _, lse = k3.lm_head_xent(X, W, label)
+    dX, dW = k3.lm_head_xent_grad(X, W, label, lse, g=g)
+    a, none = k3.lm_head_xent_grad(X, W, label, lse, g=g, need_dw=False)
+    assert none is None and torch.equal(a, dX)
+    none, b = k3.lm_head_xent_grad(X, W, label, lse, g=g, need_dx=False)
+    assert none is None and torch.equal(b, dW)
+    one = k3.lm_head_xent_grad(X, W, label, lse)
+    two = k3.lm_head_xent_grad(X, W, label, lse, g=torch.ones_like(g))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+def test_no_rows(k3):
+    X, W, g, _ = inputs(4, 64, 50, 12)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    loss, lse = k3.lm_head_xent(X[:0], W, none)
+    dX, dW = k3.lm_head_xent_grad(X[:0], W, none, lse)
+    assert loss.shape == lse.shape == (0,) and dX.shape == (0, 64) and (dW == 0).all()
+
+
+def test_repeatable_on_another_stream_and_in_a_graph(k3):
+    """Twice the same bits; on a side stream; captured once and replayed on new inputs."""
+    X, W, g, gen = inputs(270, 520, 2050, 13)
+    label = torch.randint(-1, 2050, (270,), generator=gen, device="cuda").int()
+    base = xent_all(k3, X, W, label, g)
+    again = xent_all(k3, X, W, label, g)
+    for name in base:
+        assert torch.equal(base[name], again[name])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = xent_all(k3, X, W, label, g)
+    torch.cuda.current_stream().wait_stream(side)
+    for name in base:
+        assert torch.equal(base[name], other[name])
+    Xs, ls = X.clone(), label.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = xent_all(k3, Xs, W, ls, g)
+    X2, _, _, gen = inputs(270, 520, 2050, 14)
+    l2 = torch.randint(0, 2050, (270,), generator=gen, device="cuda").int()     # now every row counts
+    for x, lab in ((X2, l2), (X, label)):
+        Xs.copy_(x)
+        ls.copy_(lab)
+        graph.replay()
+        want = xent_all(k3, x, W, lab, g)
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+    assert k3.device_status(0) == 0
+
+
+def test_a_sweep_teaches_a_head(k3):
+    """The operators as they are used together: a target's logits, their top entries, the
+    distillation of a draft head from them and both gradients, against the formulas."""
+    Xt, Wt, _, gen = inputs(90, 256, 1500, 15, spread=4.0)
+    logits = k3.matmul_bf16(Xt.float(), Wt)
+    ids, top = k3.topk_logits(logits, 24)
+    order = logits.double().cpu().sort(dim=1, descending=True, stable=True)
+    assert torch.equal(ids.cpu().long(), order.indices[:, :24])
+    X, W, g, _ = inputs(90, 128, 1500, 16)
+    got = distill_all(k3, X, W, ids, top, 2.0, g)
+    want = formula(X, W, targets_distill(ids, top, 2.0, 1500), 2.0, g)
+    for name in want:
+        holds(name, got[name], want[name])
+    # the hard-label loss on the teacher's first choice
+    got = xent_all(k3, X, W, ids[:, 0].contiguous(), g)
+    want = formula(X, W, targets_xent(ids[:, 0], 1500), 1.0, g)
+    for name in want:
+        holds(name, got[name], want[name])
