@@ -23,12 +23,16 @@
 // dW_piece = dz^T X. dz is rounded to bf16 once, relative error 2^-9 an element, the size
 // of the outputs' own rounding and independent between elements; all sums are fp32.
 //
-// One persistent CTA per SM walks tiles (10 warps):
+// One persistent CTA per SM takes units of work from a counter (10 warps):
 //   warp 0     TMA, a ring of 64-K stages: A 128 rows (16 KB), B 256 rows (32 KB)
 //   warp 1     one thread issues the MMAs (128 x 256 x 16) into one of two TMEM
 //              accumulators of 256 columns
-//   warps 2-9  epilogue of the finished accumulator while the next tile runs: warp w reads
+//   warps 2-9  epilogue of the finished accumulator while the next one fills: warp w reads
 //              the TMEM lane quarter w % 4, columns 128 ((w - 2) / 4) ..
+// The tensor core's fp32 sums are cut, not rounded, as they grow, an error with one sign; z
+// therefore leaves TMEM every 1024 of K and is summed in the epilogue's registers (for 7168
+// wide hidden states the loss is then 5.5e-7 from the 64-bit value and not 4.4e-6, at 0.3% of the time; the MMAs do not
+// wait, two accumulators alternate). dX and dW end in bf16 and stay in TMEM.
 // Every wait is bounded (a wait that gives up has waited seconds, longer than any copy in
 // flight takes); TMEM is freed on every exit path. No TMA multicast.
 #include <cuda_bf16.h>
@@ -45,110 +49,135 @@ namespace head {
 using namespace tc;
 
 constexpr int THREADS = 10 * 32;
-constexpr int BM = 128, BN = 256, KB = 64;
-constexpr int NS = 4;
-constexpr int A_BYTES = BM * KB * 2, B_BYTES = BN * KB * 2, STAGE = A_BYTES + B_BYTES;
-constexpr int SMEM = NS * STAGE + 256;
+constexpr int BM = 128, BN = 256, KB = 64; // rows a CTA, columns a unit
+constexpr int NU = 4;                      // units published ahead
+constexpr int A_BYTES = BM * KB * 2;
+constexpr int RING = 192 * 1024;           // the stages: 4 of 48 KB, or 6 of 32 KB in a pair
+constexpr int SMEM = RING + 512;
+template <int CG> struct Stage {
+    static constexpr int B_COLS = BN / CG, BYTES = A_BYTES + B_COLS * KB * 2, N = RING / BYTES;
+};
+constexpr int HALF = BN / 2;               // columns an epilogue thread holds
+constexpr int Z_CHUNK = 16;                // 64-K steps of z summed in TMEM before they join the registers
+constexpr int GROUP_D = 16 * BM;           // rows of dX and dW walked together
 constexpr int MAXK = 128;
-constexpr int ROW_PAD = 256;               // packed rows are padded to this
+constexpr int ROW_PAD = 2 * BM;            // packed rows end on a pair's tile
+constexpr int PACK_BLOCKS = 512, PACK_ROWS = 2048;
 constexpr float LOG2E = 1.4426950408889634f;
 
-enum Mode { LOSS, DZ, GRADS };
+enum Mode { LOSS, GRAD };
+enum Kind { Z, DX, DW };                   // what a unit of work forms
+
+// A vocabulary piece of the backward: ids v0 .. v0 + vc - 1, their dz [Tpad][ldz].
+struct Piece {
+    int v0, vc;
+    __nv_bfloat16 *dz;
+};
 
 struct Args {
-    int T, in, vocab;
+    int T, in;
     const int *n_live;          // rows that count
     const int *row_of;          // [T] packed row -> row
     int Tpad;
+    int x_in_place;             // X itself can be read by TMA when every row counts
     // targets, by row: entry e of row t is ids[t * K + e] (ascending), mass[t * K + e]
     const int *ids;
     const float *mass;          // nullptr: cross entropy (K = 1, mass 1)
     const int *count;           // entries of a row; nullptr: 1
     int K;
     float c;                    // log2(e) / temp
+    Piece z;                    // vc = 0: no z units in this launch
     // LOSS
     float2 *part;               // [2 * vocabulary tiles][Tpad] (max, sum), base 2
     float *zt;                  // [T][K] z of the targets
-    // DZ and GRADS: this piece of the vocabulary
-    int v0, vc;                 // first id, ids
+    // GRAD
     const float *lse, *g;       // by row; g may be nullptr (1)
     float inv_temp;
-    __nv_bfloat16 *dz;          // [Tpad][ldz]
     int ldz;
-    // GRADS
+    Piece d;                    // vc = 0: no dX and dW units in this launch
     int want_dx, want_dw, first, last;
-    float *acc;                 // [Tpad][in] dX between pieces
+    int splits, split_steps;    // dX: K splits, 64-K steps of each
+    float *acc;                 // [splits][Tpad][in] dX before its last sum
     __nv_bfloat16 *dX, *dW;
     int lddx, vec_dx;
-    int x_direct_ok;            // X itself can be read by TMA when every row counts
-    int group;                  // row tiles walked together
+    int z_before_dw;            // the longer units come first
+    int group_z;                // rows of z walked together
 };
 
 struct Maps {
     CUtensorMap x_k, xp_k;      // X and packed X, K-major boxes (64 x BM)
-    CUtensorMap w_k;            // W, K-major boxes (64 x BN)
+    CUtensorMap w_k;            // W, K-major boxes (64 x a CTA's columns)
     CUtensorMap x_mn, xp_mn, w_mn;   // 64 x 64 boxes of rows as K
-    CUtensorMap dz_k, dz_mn;    // the piece's dz, 64 x BM and 64 x 64 boxes
+    CUtensorMap dz_k, dz_mn;    // piece d's dz, 64 x BM and 64 x 64 boxes
 };
 
-// A tile of the launch: which product, its first row and column, its K steps.
-struct Tile {
-    int kind;                   // 0: z (LOSS, DZ); 1: dX; 2: dW
-    int m0, n0, steps;
-};
-
-__device__ __forceinline__ void place(int i, int mt, int nt, int group, int &m, int &n)
-{
-    // groups of row tiles; inside a group the rows run fastest, so a wave shares both the
-    // group's rows and a few column tiles through L2
-    const int per = group * nt, gr = i / per, r = i - gr * per;
-    const int size = min(group, mt - gr * group);
-    n = r / size;
-    m = gr * group + (r - n * size);
-}
-
-template <int MODE>
-struct Walk {
-    int n, mt, nt, mt2, nt2, first2, total, steps_k, steps_v, steps_n;
-    __device__ __forceinline__ Walk(const Args &a, int n_live)
+// A unit: a 128 CG x 256 tile of one product (or of one K split of it), worked on by a CTA
+// (CG = 1) or a pair of them. The producer publishes it to its CTA's warps as four words.
+struct Unit {
+    int kind, m0, n0, split, step0, steps;
+    __device__ __forceinline__ int4 words() const { return make_int4(kind | (split << 4), m0, n0, steps); }
+    static __device__ __forceinline__ Unit of(const int4 &w)
     {
-        n = n_live;
-        mt = (n + BM - 1) / BM;
-        if (MODE != GRADS) {
-            nt = (a.vc + BN - 1) / BN;
-            steps_k = (a.in + KB - 1) / KB;
-            first2 = total = mt * nt;
-            mt2 = nt2 = steps_v = steps_n = 0;
-        } else {
-            nt = nt2 = (a.in + BN - 1) / BN;
-            mt2 = (a.vc + BM - 1) / BM;
-            steps_k = 0;
-            steps_v = (a.vc + KB - 1) / KB;
-            steps_n = (n + KB - 1) / KB;
-            first2 = a.want_dx ? mt * nt : 0;
-            total = first2 + (a.want_dw ? mt2 * nt2 : 0);
-        }
+        return Unit{w.x < 0 ? -1 : (w.x & 15), w.y, w.z, w.x >> 4, 0, w.w};
     }
-    __device__ __forceinline__ Tile at(int i, const Args &a) const
+};
+
+template <int MODE, int CG>
+struct Units {
+    static constexpr int TM = BM * CG;
+    int n_dx, n_dw, n_z, total;
+    int mt, nt_in, nt_z, mt_w, steps_in, steps_v, steps_n;
+    __device__ __forceinline__ Units(const Args &a, int n)
     {
-        Tile t;
-        int m, c;
-        if (MODE != GRADS) {
-            t.kind = 0;
-            place(i, mt, nt, a.group, m, c);
-            t.steps = steps_k;
-        } else if (i < first2) {
-            t.kind = 1;
-            place(i, mt, nt, a.group, m, c);
-            t.steps = steps_v;
+        mt = (n + TM - 1) / TM;
+        nt_in = (a.in + BN - 1) / BN;
+        nt_z = (a.z.vc + BN - 1) / BN;
+        mt_w = (a.d.vc + TM - 1) / TM;
+        steps_in = (a.in + KB - 1) / KB;
+        steps_v = (a.d.vc + KB - 1) / KB;
+        steps_n = (n + KB - 1) / KB;
+        n_z = mt * nt_z;
+        n_dx = MODE == GRAD && a.want_dx && a.d.vc ? mt * nt_in * a.splits : 0;
+        n_dw = MODE == GRAD && a.want_dw ? mt_w * nt_in : 0;
+        total = n_dx + n_dw + n_z;
+    }
+    // groups of row tiles; inside a group the rows run fastest, so the units in flight share
+    // both the group's rows and a few column tiles through L2
+    static __device__ __forceinline__ void place(int i, int m_tiles, int n_tiles, int group, int &m, int &n)
+    {
+        const int per = group * n_tiles, gr = i / per, r = i - gr * per;
+        const int size = min(group, m_tiles - gr * group);
+        n = r / size;
+        m = gr * group + (r - n * size);
+    }
+    __device__ __forceinline__ Unit at(int i, const Args &a) const
+    {
+        Unit u;
+        int m = 0, c = 0;
+        u.split = 0;
+        u.step0 = 0;
+        if (MODE == GRAD && i < n_dx) {
+            u.kind = DX;
+            u.split = i / (mt * nt_in);
+            place(i - u.split * (mt * nt_in), mt, nt_in, GROUP_D / TM, m, c);
+            u.step0 = u.split * a.split_steps;
+            u.steps = max(0, min(a.split_steps, steps_v - u.step0));
         } else {
-            t.kind = 2;
-            place(i - first2, mt2, nt2, a.group, m, c);
-            t.steps = steps_n;
+            i -= n_dx;
+            const bool z = MODE == LOSS || (a.z_before_dw ? i < n_z : i >= n_dw);
+            if (z) {
+                u.kind = Z;
+                place(MODE == LOSS || a.z_before_dw ? i : i - n_dw, mt, nt_z, a.group_z / TM, m, c);
+                u.steps = steps_in;
+            } else {
+                u.kind = DW;
+                place(a.z_before_dw ? i - n_z : i, mt_w, nt_in, GROUP_D / TM, m, c);
+                u.steps = steps_n;
+            }
         }
-        t.m0 = m * BM;
-        t.n0 = c * BN;
-        return t;
+        u.m0 = m * TM;
+        u.n0 = c * BN;
+        return u;
     }
 };
 
@@ -164,6 +193,64 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32])
         : "r"(taddr)
         : "memory");
 }
+// The pair's forms (CG = 2, a cluster of two CTAs, rank 0 leads): loads signal the leader's
+// barrier, the leader's MMAs read both CTAs' shared memory and write both's TMEM, a commit
+// arrives at the barrier of the same place in both.
+__device__ __forceinline__ uint32_t at_rank0(uint32_t saddr)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(saddr));
+    return r;
+}
+template <int CG>
+__device__ __forceinline__ void load2d(uint32_t dst, const CUtensorMap *m, int x, int y, uint32_t bar)
+{
+    if (CG == 1) {
+        tma2d(dst, m, x, y, bar);
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+            "{%2, %3}], [%4];" ::"r"(dst),
+            "l"(m), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t more)
+{
+    if (CG == 1) {
+        mma_ss(d, ad, bd, idesc, more);
+    } else {
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(more)
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+    if (CG == 1) {
+        mma_commit(bar);
+    } else {
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                bar),
+            "h"((uint16_t)3)
+            : "memory");
+    }
+}
+// every thread of the cluster; orders what came before it for what comes after
+template <int CG>
+__device__ __forceinline__ void sync_all()
+{
+    if (CG == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
@@ -175,18 +262,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t *>(&h);
 }
-__device__ __forceinline__ float pick(const uint32_t (&v)[32], int j)
+// the first of a row's entries at or past id v
+__device__ __forceinline__ int first_entry(const int *ids, int cnt, int v)
 {
-    float z = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-        if (i == j) z = __uint_as_float(v[i]);
-    return z;
-}
-// the first of row t's entries at or past id v
-__device__ __forceinline__ int first_entry(const Args &a, int t, int cnt, int v)
-{
-    const int *ids = a.ids + (size_t)t * a.K;
     int lo = 0, hi = cnt;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -196,18 +274,92 @@ __device__ __forceinline__ int first_entry(const Args &a, int t, int cnt, int v)
     return lo;
 }
 
-template <int MODE>
+// One unit's z in registers: the thread's row, HALF columns from col0 of the piece. What the row
+// needs was fetched before the products were done.
+struct RowTargets {
+    const int *ids;
+    int e, cnt, next;           // the next entry, entries, the next entry's column in the piece
+    __device__ __forceinline__ void start(const Args &a, int t, bool live, int col0)
+    {
+        ids = a.ids + (size_t)t * a.K;
+        cnt = live ? (a.count ? a.count[t] : 1) : 0;
+        e = first_entry(ids, cnt, a.z.v0 + col0);
+        next = e < cnt ? ids[e] - a.z.v0 : 0x7fffffff;
+    }
+    __device__ __forceinline__ void step(const Args &a)
+    {
+        e++;
+        next = e < cnt ? ids[e] - a.z.v0 : 0x7fffffff;
+    }
+};
+
+__device__ __forceinline__ void loss_epilogue(const Args &a, float (&z)[HALF], RowTargets &tg, int t, int row,
+                                              bool live, int col0)
+{
+#pragma unroll
+    for (int c0 = 0; c0 < HALF; c0 += 32)
+        while (tg.next < col0 + c0 + 32) {
+            const uint32_t at = 1u << (tg.next - col0 - c0);   // a bit, so that z stays in registers
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (at & (1u << j)) v = z[c0 + j];
+            a.zt[(size_t)t * a.K + tg.e] = v;
+            tg.step(a);
+        }
+    const int left = a.z.vc - col0;
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < HALF; j++) {
+        z[j] = j < left ? z[j] * a.c : -INFINITY;
+        mx[j & 3] = fmaxf(mx[j & 3], z[j]);
+    }
+    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), ref = m == -INFINITY ? 0.0f : m;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < HALF; j++) s[j & 3] += ex2(z[j] - ref);
+    if (live) a.part[(size_t)(col0 / HALF) * a.Tpad + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
+}
+
+__device__ __forceinline__ void dz_epilogue(const Args &a, float (&z)[HALF], RowTargets &tg, int t, int row,
+                                            bool live, int col0, float l2, float gt)
+{
+#pragma unroll
+    for (int j = 0; j < HALF; j++) z[j] = ex2(fmaf(z[j], a.c, -l2));
+#pragma unroll
+    for (int c0 = 0; c0 < HALF; c0 += 32)
+        while (tg.next < col0 + c0 + 32) {
+            const uint32_t at = 1u << (tg.next - col0 - c0);   // a bit, so that z stays in registers
+            const float q = a.mass ? a.mass[(size_t)t * a.K + tg.e] : 1.0f;
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (at & (1u << j)) z[c0 + j] -= q;
+            tg.step(a);
+        }
+    // rows of the tile past the live ones are zeros: dW sums over them
+    uint4 *dst = reinterpret_cast<uint4 *>(a.z.dz + (size_t)row * a.ldz + col0);
+#pragma unroll
+    for (int j = 0; j < HALF; j += 8) {
+        uint4 o = make_uint4(0u, 0u, 0u, 0u);
+        if (live)
+            o = make_uint4(pack_bf16(z[j] * gt, z[j + 1] * gt), pack_bf16(z[j + 2] * gt, z[j + 3] * gt),
+                           pack_bf16(z[j + 4] * gt, z[j + 5] * gt), pack_bf16(z[j + 6] * gt, z[j + 7] * gt));
+        dst[j / 8] = o;
+    }
+}
+
+template <int MODE, int CG>
 __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant__ Maps maps, const Args a)
 {
+    using St = Stage<CG>;
+    constexpr int NS = St::N;
     extern __shared__ __align__(1024) unsigned char smem[];
-    if ((s_addr(smem) & 1023u) != 0u) {   // never expected: refuse rather than mis-swizzle
-        if (threadIdx.x == 0) flag(DEV_BAD_INDEX);
-        return;
-    }
-    uint64_t *b_full = reinterpret_cast<uint64_t *>(smem + NS * STAGE), *b_empty = b_full + NS;
-    uint64_t *b_done = b_empty + NS, *b_free = b_done + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(b_free + 2);
+    uint64_t *b_full = reinterpret_cast<uint64_t *>(smem + RING), *b_empty = b_full + NS;
+    uint64_t *b_done = b_empty + NS, *b_free = b_done + 2, *b_unit = b_free + 2, *b_took = b_unit + NU;
+    int4 *unit_slot = reinterpret_cast<int4 *>(b_took + NU);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(unit_slot + NU);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CG == 1 ? 0 : blockIdx.x & 1;   // in the cluster of two
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; s++) {
             bar_init(s_addr(&b_full[s]), 1);
@@ -215,178 +367,197 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
         }
         for (int d = 0; d < 2; d++) {
             bar_init(s_addr(&b_done[d]), 1);
-            bar_init(s_addr(&b_free[d]), 8);       // the epilogue warps
+            bar_init(s_addr(&b_free[d]), 8 * CG);  // the epilogue warps
+        }
+        for (int u = 0; u < NU; u++) {
+            bar_init(s_addr(&b_unit[u]), 1);
+            bar_init(s_addr(&b_took[u]), rank == 0 ? 9 : 8);   // the MMA thread and the epilogue warps
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s_addr(tmem_slot))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s_addr(tmem_slot))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s_addr(tmem_slot))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
     }
     fence_before();
-    __syncthreads();
+    sync_all<CG>();
     fence_after();
     const uint32_t tmem = *tmem_slot;
     const int n_live = *a.n_live;
-    const Walk<MODE> walk(a, n_live);
-    const bool direct = a.x_direct_ok && n_live == a.T;
     bool failed = false;
 
     if (warp == 0) {
         if (lane == 0) {
-            const CUtensorMap *xk = direct ? &maps.x_k : &maps.xp_k, *xmn = direct ? &maps.x_mn : &maps.xp_mn;
-            int item = 0;
-            for (int i = blockIdx.x; i < walk.total && !failed; i += gridDim.x) {
-                const Tile t = walk.at(i, a);
+            const bool in_place = a.x_in_place && n_live == a.T;
+            const CUtensorMap *xk = in_place ? &maps.x_k : &maps.xp_k, *xmn = in_place ? &maps.x_mn : &maps.xp_mn;
+            const Units<MODE, CG> units(a, n_live);
+            int item = 0, n_units = 0;
+            for (int i = blockIdx.x / CG; !failed; i += gridDim.x / CG) {
+                const int slot = n_units % NU;
+                if (!bar_wait(s_addr(&b_took[slot]), (uint32_t)((n_units / NU) & 1) ^ 1u)) { failed = true; break; }
+                const bool end = i >= units.total;
+                Unit t{};
+                if (!end) t = units.at(i, a);
+                unit_slot[slot] = end ? make_int4(-1, 0, 0, 0) : t.words();
+                bar_arrive(s_addr(&b_unit[slot]));
+                n_units++;
+                if (end) break;
+                const int m0 = t.m0 + rank * BM, n0 = t.n0 + rank * St::B_COLS;
                 for (int ks = 0; ks < t.steps; ks++, item++) {
                     const int st = item % NS;
                     if (!bar_wait(s_addr(&b_empty[st]), (uint32_t)((item / NS) & 1) ^ 1u)) { failed = true; break; }
-                    const uint32_t sa = s_addr(smem + st * STAGE), sb = sa + A_BYTES, full = s_addr(&b_full[st]);
-                    bar_expect(full, STAGE);
-                    const int k = ks * KB;
-                    if (MODE != GRADS) {
-                        tma2d(sa, xk, k, t.m0, full);
-                        tma2d(sb, &maps.w_k, k, a.v0 + t.n0, full);
-                    } else if (t.kind == 1) {
-                        tma2d(sa, &maps.dz_k, k, t.m0, full);
+                    const uint32_t sa = s_addr(smem + st * St::BYTES), sb = sa + A_BYTES;
+                    uint32_t full = s_addr(&b_full[st]);
+                    if (rank == 0) bar_expect(full, CG * St::BYTES);
+                    if (CG > 1) full = at_rank0(full);
+                    const int k = (t.step0 + ks) * KB;
+                    if (MODE == LOSS || t.kind == Z) {
+                        load2d<CG>(sa, xk, k, m0, full);
+                        load2d<CG>(sb, &maps.w_k, k, a.z.v0 + n0, full);
+                    } else if (t.kind == DX) {
+                        load2d<CG>(sa, &maps.dz_k, k, m0, full);
 #pragma unroll
-                        for (int b = 0; b < BN / 64; b++)
-                            tma2d(sb + b * 8192, &maps.w_mn, t.n0 + b * 64, a.v0 + k, full);
+                        for (int b = 0; b < St::B_COLS / 64; b++)
+                            load2d<CG>(sb + b * 8192, &maps.w_mn, n0 + b * 64, a.d.v0 + k, full);
                     } else {
 #pragma unroll
                         for (int b = 0; b < BM / 64; b++)
-                            tma2d(sa + b * 8192, &maps.dz_mn, t.m0 + b * 64, k, full);
+                            load2d<CG>(sa + b * 8192, &maps.dz_mn, m0 + b * 64, k, full);
 #pragma unroll
-                        for (int b = 0; b < BN / 64; b++) tma2d(sb + b * 8192, xmn, t.n0 + b * 64, k, full);
+                        for (int b = 0; b < St::B_COLS / 64; b++)
+                            load2d<CG>(sb + b * 8192, xmn, n0 + b * 64, k, full);
                     }
                 }
             }
             if (failed) flag(DEV_TIMEOUT);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             int item = 0, use = 0;
-            for (int i = blockIdx.x; i < walk.total && !failed; i += gridDim.x, use++) {
-                const Tile t = walk.at(i, a);
-                const int d = use & 1;
-                if (!bar_wait(s_addr(&b_free[d]), (uint32_t)((use >> 1) & 1) ^ 1u)) { failed = true; break; }
-                fence_after();
-                const uint32_t dt = tmem + (uint32_t)(d * BN);
-                // A and B: K-major for z; dX takes W as rows of K, dW both operands so
-                const uint32_t idesc = bf16_idesc(BN, t.kind >= 1) | (t.kind == 2 ? (1u << 15) : 0u);
-                const uint32_t da = t.kind == 2 ? 2048u >> 4 : 32u >> 4, db = t.kind >= 1 ? 2048u >> 4 : 32u >> 4;
-                for (int ks = 0; ks < t.steps; ks++, item++) {
-                    const int st = item % NS;
-                    if (!bar_wait(s_addr(&b_full[st]), (uint32_t)((item / NS) & 1))) { failed = true; break; }
+            for (int n_units = 0; !failed; n_units++) {
+                const int slot = n_units % NU;
+                if (!bar_wait(s_addr(&b_unit[slot]), (uint32_t)((n_units / NU) & 1))) { failed = true; break; }
+                const Unit t = Unit::of(unit_slot[slot]);
+                bar_arrive(s_addr(&b_took[slot]));
+                if (t.kind < 0) break;
+                // A and B are K-major for z; dX takes W as rows of K, dW both operands so
+                const bool b_mn = MODE == GRAD && t.kind != Z, a_mn = MODE == GRAD && t.kind == DW;
+                const uint32_t idesc = (bf16_idesc(BN, b_mn) + ((uint32_t)(CG - 1) << 27)) | (a_mn ? (1u << 15) : 0u);
+                const uint32_t da = a_mn ? 2048u >> 4 : 32u >> 4, db = b_mn ? 2048u >> 4 : 32u >> 4;
+                const int chunk = b_mn ? t.steps : Z_CHUNK;
+                for (int ks = 0; ks < t.steps && !failed; use++) {
+                    const int d = use & 1, end = min(t.steps, ks + chunk);
+                    if (!bar_wait(s_addr(&b_free[d]), (uint32_t)((use >> 1) & 1) ^ 1u)) { failed = true; break; }
                     fence_after();
-                    const uint32_t sa = s_addr(smem + st * STAGE), sb = sa + A_BYTES;
-                    const uint64_t ad = t.kind == 2 ? sw128_mn_desc(sa, 8192) : sw128_desc(sa);
-                    const uint64_t bd = t.kind >= 1 ? sw128_mn_desc(sb, 8192) : sw128_desc(sb);
+                    const uint32_t dt = tmem + (uint32_t)(d * BN);
+                    for (uint32_t more = 0; ks < end; ks++, item++) {
+                        const int st = item % NS;
+                        if (!bar_wait(s_addr(&b_full[st]), (uint32_t)((item / NS) & 1))) { failed = true; break; }
+                        fence_after();
+                        const uint32_t sa = s_addr(smem + st * St::BYTES), sb = sa + A_BYTES;
+                        const uint64_t ad = a_mn ? sw128_mn_desc(sa, 8192) : sw128_desc(sa);
+                        const uint64_t bd = b_mn ? sw128_mn_desc(sb, 8192) : sw128_desc(sb);
 #pragma unroll
-                    for (int u = 0; u < KB / 16; u++)
-                        mma_ss(dt, ad + u * da, bd + u * db, idesc, (uint32_t)(ks > 0 || u > 0));
-                    mma_commit(s_addr(&b_empty[st]));
+                        for (int u = 0; u < KB / 16; u++) {
+                            mma<CG>(dt, ad + u * da, bd + u * db, idesc, more);
+                            more = 1;
+                        }
+                        commit<CG>(s_addr(&b_empty[st]));
+                    }
+                    if (!failed) commit<CG>(s_addr(&b_done[d]));
                 }
-                if (failed) break;
-                if (t.steps > 0) mma_commit(s_addr(&b_done[d]));
-                else bar_arrive(s_addr(&b_done[d]));
             }
             if (failed) flag(DEV_TIMEOUT);
         }
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
-        const int r = q * 32 + lane;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         int use = 0;
-        for (int i = blockIdx.x; i < walk.total && !failed; i += gridDim.x, use++) {
-            const Tile t = walk.at(i, a);
-            const int d = use & 1;
-            const int row = t.m0 + r;              // packed row (z, dX) or id of the piece (dW)
-            const int col0 = t.n0 + half * (BN / 2);
-            const uint32_t src = tmem + lanes + (uint32_t)(d * BN + half * (BN / 2));
-            if constexpr (MODE != GRADS) {
-                // what the row needs is fetched while the tile's products still run
+        // the next finished accumulator
+        auto finished = [&]() {
+            if (!bar_wait(s_addr(&b_done[use & 1]), (uint32_t)((use >> 1) & 1))) return false;
+            fence_after();
+            return true;
+        };
+        // the leader's MMAs may write this accumulator again
+        auto release = [&]() {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                const uint32_t b = s_addr(&b_free[use & 1]);
+                if (CG == 1 || rank == 0) bar_arrive(b);
+                else
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank0(b))
+                                 : "memory");
+            }
+            use++;
+        };
+        for (int n_units = 0; !failed; n_units++) {
+            const int slot = n_units % NU;
+            if (!bar_wait(s_addr(&b_unit[slot]), (uint32_t)((n_units / NU) & 1))) { failed = true; break; }
+            const Unit t = Unit::of(unit_slot[slot]);
+            __syncwarp();
+            if (lane == 0) bar_arrive(s_addr(&b_took[slot]));
+            if (t.kind < 0) break;
+            const int row = t.m0 + rank * BM + q * 32 + lane;   // packed row (z, dX) or id of the piece (dW)
+            const int col0 = t.n0 + half * HALF;
+            const uint32_t src = tmem + lanes + (uint32_t)(half * HALF);
+            if (MODE == LOSS || t.kind == Z) {
+                // what the row needs is fetched while the unit's products run
                 const bool live = row < n_live;
                 const int tr = live ? a.row_of[row] : 0;
-                const int cnt = live ? (a.count ? a.count[tr] : 1) : 0;
-                const int *ids = a.ids + (size_t)tr * a.K;
-                int e = cnt > 0 ? first_entry(a, tr, cnt, a.v0 + col0) : 0;
-                int next = e < cnt ? ids[e] - a.v0 : 0x7fffffff;
+                RowTargets tg;
+                tg.start(a, tr, live, col0);
                 float l2 = 0.0f, gt = 0.0f;
-                if (MODE == DZ && live) {
+                if (MODE == GRAD && live) {
                     l2 = a.lse[tr] * LOG2E;
                     gt = (a.g ? a.g[tr] : 1.0f) * a.inv_temp;
                 }
-                if (!bar_wait(s_addr(&b_done[d]), (uint32_t)((use >> 1) & 1))) { failed = true; break; }
-                fence_after();
-                float mx = -INFINITY, sum = 0.0f;
-                for (int c0 = 0; c0 < BN / 2; c0 += 32) {
-                    uint32_t v[32];
-                    __syncwarp();                  // the targets' branches below part the lanes
-                    tmem_ld32(src + (uint32_t)c0, v);
-                    tmem_wait_ld();
-                    const int col = col0 + c0;
-                    if constexpr (MODE == LOSS) {
-                        while (next < col + 32) {
-                            a.zt[(size_t)tr * a.K + e] = pick(v, next - col);
-                            e++;
-                            next = e < cnt ? ids[e] - a.v0 : 0x7fffffff;
-                        }
-                        const int left = a.vc - col;
-                        float cm = -INFINITY;
+                float z[HALF];
 #pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            const float z = j < left ? __uint_as_float(v[j]) * a.c : -INFINITY;
-                            v[j] = __float_as_uint(z);
-                            cm = fmaxf(cm, z);
-                        }
-                        const float mn = fmaxf(mx, cm), ref = mn == -INFINITY ? 0.0f : mn;
-                        float cs = 0.0f;
+                for (int j = 0; j < HALF; j++) z[j] = 0.0f;
+                __syncwarp();
+#pragma unroll 1
+                for (int ks = 0; ks < t.steps; ks += Z_CHUNK) {
+                    if (!finished()) { failed = true; break; }
+                    const uint32_t at = src + (uint32_t)((use & 1) * BN);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) cs += ex2(__uint_as_float(v[j]) - ref);
-                        sum = sum * ex2(mx - ref) + cs;
-                        mx = mn;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            v[j] = __float_as_uint(live ? ex2(__uint_as_float(v[j]) * a.c - l2) : 0.0f);
-                        while (next < col + 32) {
-                            const float q_e = a.mass ? a.mass[(size_t)tr * a.K + e] : 1.0f;
-#pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (j == next - col) v[j] = __float_as_uint(__uint_as_float(v[j]) - q_e);
-                            e++;
-                            next = e < cnt ? ids[e] - a.v0 : 0x7fffffff;
-                        }
-                        uint32_t o[16];
+                    for (int c0 = 0; c0 < HALF; c0 += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(at + (uint32_t)c0, v);
+                        tmem_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 16; j++)
-                            o[j] = live ? pack_bf16(__uint_as_float(v[2 * j]) * gt, __uint_as_float(v[2 * j + 1]) * gt)
-                                        : 0u;
-                        if (col < a.ldz) {          // ldz is a multiple of 64
-                            uint4 *dst = reinterpret_cast<uint4 *>(a.dz + (size_t)row * a.ldz + col);
-#pragma unroll
-                            for (int j = 0; j < 4; j++) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                        }
+                            z[c0 + j] += __uint_as_float(v[j]);
                     }
+                    release();
                 }
-                if (MODE == LOSS && live) a.part[(size_t)(col0 / (BN / 2)) * a.Tpad + row] = make_float2(mx, sum);
+                if (failed) break;
+                if (MODE == LOSS) loss_epilogue(a, z, tg, tr, row, live, col0);
+                else dz_epilogue(a, z, tg, tr, row, live, col0, l2, gt);
+                __syncwarp();
             } else {
-                if (!bar_wait(s_addr(&b_done[d]), (uint32_t)((use >> 1) & 1))) { failed = true; break; }
-                fence_after();
-                const bool dx = t.kind == 1;
-                const bool live = dx ? row < n_live : row < a.vc;
-                float *acc = a.acc + (size_t)row * a.in;
+                const bool dx = t.kind == DX;
+                const bool live = dx ? row < n_live : row < a.d.vc;
+                const bool sum = dx && (a.splits > 1 || !a.last), add = dx && !a.first;
+                float *acc = a.acc + ((size_t)t.split * a.Tpad + row) * a.in;
                 __nv_bfloat16 *out = nullptr;
-                if (live) out = dx ? a.dX + (size_t)a.row_of[row] * a.lddx : a.dW + (size_t)(a.v0 + row) * a.in;
+                if (live) out = dx ? a.dX + (size_t)a.row_of[row] * a.lddx : a.dW + (size_t)(a.d.v0 + row) * a.in;
                 const bool vec = dx ? a.vec_dx : 1;
-                for (int c0 = 0; c0 < BN / 2; c0 += 32) {
+                if (t.steps > 0 && !finished()) { failed = true; break; }
+                for (int c0 = 0; c0 < HALF; c0 += 32) {
                     const int col = col0 + c0;
                     uint32_t v[32];
                     __syncwarp();
                     if (t.steps > 0) {
-                        tmem_ld32(src + (uint32_t)c0, v);
+                        tmem_ld32(src + (uint32_t)((use & 1) * BN + c0), v);
                         tmem_wait_ld();
                     } else {
 #pragma unroll
@@ -398,13 +569,13 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                         float f[8];
 #pragma unroll
                         for (int u = 0; u < 8; u++) f[u] = __uint_as_float(v[j + u]);
-                        if (dx && !a.first) {
+                        if (add) {
                             const float4 p0 = *reinterpret_cast<const float4 *>(acc + col + j);
                             const float4 p1 = *reinterpret_cast<const float4 *>(acc + col + j + 4);
                             f[0] += p0.x; f[1] += p0.y; f[2] += p0.z; f[3] += p0.w;
                             f[4] += p1.x; f[5] += p1.y; f[6] += p1.z; f[7] += p1.w;
                         }
-                        if (dx && !a.last) {
+                        if (sum) {
                             *reinterpret_cast<float4 *>(acc + col + j) = make_float4(f[0], f[1], f[2], f[3]);
                             *reinterpret_cast<float4 *>(acc + col + j + 4) = make_float4(f[4], f[5], f[6], f[7]);
                         } else if (vec) {
@@ -417,18 +588,45 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                         }
                     }
                 }
+                __syncwarp();
+                if (t.steps > 0) release();
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(s_addr(&b_free[d]));
         }
         if (failed && lane == 0) flag(DEV_TIMEOUT);
     }
     fence_before();
-    __syncthreads();
+    __syncwarp();
+    sync_all<CG>();
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if (CG == 1)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// dX = the splits' sums in order, as bf16: block (x, y) 8 columns a thread of packed row y
+__global__ void __launch_bounds__(128) sum_splits_kernel(__nv_bfloat16 *__restrict__ dX, int lddx, int vec,
+                                                         const float *__restrict__ acc, int splits, int Tpad, int in,
+                                                         const int *__restrict__ row_of, const int *__restrict__ n_live)
+{
+    const int row = blockIdx.y, col = (blockIdx.x * 128 + threadIdx.x) * 8;
+    if (row >= *n_live || col >= in) return;
+    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = 0; s < splits; s++) {
+        const float4 *p = reinterpret_cast<const float4 *>(acc + ((size_t)s * Tpad + row) * in + col);
+        const float4 p0 = p[0], p1 = p[1];
+        f[0] += p0.x; f[1] += p0.y; f[2] += p0.z; f[3] += p0.w;
+        f[4] += p1.x; f[5] += p1.y; f[6] += p1.z; f[7] += p1.w;
+    }
+    __nv_bfloat16 *out = dX + (size_t)row_of[row] * lddx + col;
+    if (vec) {
+        *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]),
+                                                     pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    } else {
+#pragma unroll
+        for (int u = 0; u < 8; u++) out[u] = __float2bfloat16_rn(f[u]);
     }
 }
 
@@ -491,79 +689,82 @@ __global__ void __launch_bounds__(MAXK) teacher_kernel(int *__restrict__ s_ids, 
     }
 }
 
-// One block numbers the rows that count, in order: place[t] (-1: none), row_of[place] = t.
-__global__ void __launch_bounds__(1024) plan_kernel(int *__restrict__ place, int *__restrict__ row_of,
-                                                    int *__restrict__ n_live, const int *__restrict__ label,
-                                                    const int *__restrict__ count, int T, int vocab)
+// Numbers the rows that count, in order (row_of[place] = t, *n_live), copies their hidden
+// states to their places and writes zeros for the others' outputs. Each block takes `rows`
+// rows and counts the live ones before them itself (T * 4 bytes from L2, at most PACK_BLOCKS
+// blocks), so one launch does it. When every row counts and X can be read in place nothing
+// is copied; else the rows from the last packed one to the end of its tile become zeros.
+__global__ void __launch_bounds__(256) pack_kernel(int *__restrict__ row_of, int *__restrict__ n_live,
+                                                   __nv_bfloat16 *__restrict__ Xp, float *__restrict__ loss,
+                                                   float *__restrict__ lse, __nv_bfloat16 *__restrict__ dX, int lddx,
+                                                   const uint16_t *__restrict__ X, int ldx, int in_place,
+                                                   const int *__restrict__ label, const int *__restrict__ count,
+                                                   int T, int in, int vocab, int rows)
 {
-    __shared__ int warp_n[32];
-    __shared__ int base;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) base = 0;
+    __shared__ int red[2][8];
+    __shared__ int place[PACK_ROWS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int t0 = blockIdx.x * rows, t1 = min(T, t0 + rows);
+    auto counts = [&](int t) {
+        if (!label) return count[t] > 0;
+        const int l = label[t];
+        return l >= 0 && l < vocab;
+    };
+    int before = 0, total = 0;
+    for (int t = tid; t < T; t += 256) {
+        const int c = counts(t);
+        total += c;
+        before += t < t0 ? c : 0;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (lane == 0) { red[0][warp] = before; red[1][warp] = total; }
     __syncthreads();
-    for (int t0 = 0; t0 < T; t0 += 1024) {
-        const int t = t0 + threadIdx.x;
-        bool live = false;
-        if (t < T) {
-            if (label) {
-                const int l = label[t];
-                if (l >= vocab) flag(DEV_BAD_INDEX);
-                live = l >= 0 && l < vocab;
-            } else {
-                live = count[t] > 0;
-            }
+    before = total = 0;
+#pragma unroll
+    for (int w = 0; w < 8; w++) { before += red[0][w]; total += red[1][w]; }
+    if (warp == 0) {
+        for (int b = t0; b < t1; b += 32) {
+            const int t = b + lane;
+            const bool live = t < t1 && counts(t);
+            if (t < t1 && label && label[t] >= vocab) flag(DEV_BAD_INDEX);
+            const unsigned m = __ballot_sync(0xffffffffu, live);
+            const int p = before + __popc(m & ((1u << lane) - 1));
+            if (t < t1) place[t - t0] = live ? p : -1;
+            if (live) row_of[p] = t;
+            before += __popc(m);
         }
-        const unsigned m = __ballot_sync(0xffffffffu, live);
-        if (lane == 0) warp_n[warp] = __popc(m);
-        __syncthreads();
-        int before = base;
-        for (int w = 0; w < warp; w++) before += warp_n[w];
-        const int p = before + __popc(m & ((1u << lane) - 1));
-        if (t < T) place[t] = live ? p : -1;
-        if (live) row_of[p] = t;
-        __syncthreads();
-        if (threadIdx.x == 1023) base = before + __popc(m);
-        __syncthreads();
     }
-    if (threadIdx.x == 0) *n_live = base;
-}
-
-// Block t < T: row t's hidden state to its packed place, or, for a row that does not count,
-// zeros to its outputs. Blocks T ..: the zero rows behind the last packed one. Nothing is
-// copied when every row counts and X can be read in place.
-__global__ void __launch_bounds__(256) gather_kernel(__nv_bfloat16 *__restrict__ Xp, float *__restrict__ loss,
-                                                     float *__restrict__ lse, __nv_bfloat16 *__restrict__ dX, int lddx,
-                                                     const uint16_t *__restrict__ X, int ldx,
-                                                     const int *__restrict__ place, const int *__restrict__ n_live,
-                                                     int T, int in, int Tpad, int direct_ok)
-{
-    const int n = *n_live;
-    const bool copy = !(direct_ok && n == T);
+    if (blockIdx.x == 0 && tid == 0) *n_live = total;
+    __syncthreads();
+    const bool copy = !(in_place && total == T);
     uint16_t *xp = reinterpret_cast<uint16_t *>(Xp);
-    if ((int)blockIdx.x >= T) {
-        const int p = n + (int)blockIdx.x - T;
-        if (copy && p < Tpad)
-            for (int i = threadIdx.x; i < in; i += 256) xp[(size_t)p * in + i] = 0;
-        return;
-    }
-    const int t = blockIdx.x, p = place[t];
-    if (p >= 0) {
-        if (!copy) return;
-        const uint16_t *x = X + (size_t)t * ldx;
-        if (direct_ok) {                           // rows 16-byte aligned
-            for (int i = threadIdx.x; i < in / 8; i += 256)
-                reinterpret_cast<uint4 *>(xp + (size_t)p * in)[i] = reinterpret_cast<const uint4 *>(x)[i];
-        } else {
-            for (int i = threadIdx.x; i < in; i += 256) xp[(size_t)p * in + i] = x[i];
+    for (int t = t0 + warp; t < t1; t += 8) {
+        const int p = place[t - t0];
+        if (p >= 0) {
+            if (!copy) continue;
+            const uint16_t *x = X + (size_t)t * ldx;
+            if (in_place) {                        // rows 16-byte aligned
+#pragma unroll 4
+                for (int i = lane; i < in / 8; i += 32)
+                    reinterpret_cast<uint4 *>(xp + (size_t)p * in)[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
+            } else {
+#pragma unroll 4
+                for (int i = lane; i < in; i += 32) xp[(size_t)p * in + i] = __ldg(x + i);
+            }
+            continue;
         }
-        return;
+        if (loss && lane == 0) {
+            loss[t] = 0.0f;
+            lse[t] = 0.0f;
+        }
+        if (dX)
+            for (int i = lane; i < in; i += 32) dX[(size_t)t * lddx + i] = __float2bfloat16_rn(0.0f);
     }
-    if (loss && threadIdx.x == 0) {
-        loss[t] = 0.0f;
-        lse[t] = 0.0f;
-    }
-    if (dX)
-        for (int i = threadIdx.x; i < in; i += 256) dX[(size_t)t * lddx + i] = __float2bfloat16_rn(0.0f);
+    if (copy)
+        for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + ROW_PAD - 1) / ROW_PAD * ROW_PAD; p += (int)gridDim.x * 8)
+            for (int i = lane; i < in / 8; i += 32)
+                reinterpret_cast<uint4 *>(xp + (size_t)p * in)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // 32 packed rows a block, 32 threads a row: the tile halves' statistics joined in double.
@@ -661,26 +862,70 @@ constexpr long long MAX_T = 1 << 20, MAX_VOCAB = 1 << 24, MAX_IN = 1 << 16;
 static size_t a256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct Plan {
-    int Tpad, tiles, piece, ldz;       // vocabulary tiles; ids per piece of the backward
+    int cg;                            // CTAs that share a unit of the backward
+    int Tpad, tiles, piece, pieces;    // vocabulary tiles; ids per piece of the backward; pieces
+    int splits, split_steps;           // of dX's K (a piece)
+    size_t dz_bytes;                   // of one piece
 };
 
-static Plan plan(int T, int vocab)
+// The steps of the busiest worker when units of three kinds are dealt out in turn: each kind
+// gives every worker n / workers units and one more to the n % workers after its start, so
+// the busiest is a worker at which some kind starts.
+static double busiest(const long long (&n)[3], const double (&cost)[3], int workers)
+{
+    const int start[3] = {0, (int)(n[0] % workers), (int)((n[0] + n[1]) % workers)};
+    double most = 0.0;
+    for (int w : start) {
+        double t = 0.0;
+        for (int k = 0; k < 3; k++)
+            t += cost[k] * (double)(n[k] / workers + ((w - start[k] + workers) % workers < n[k] % workers ? 1 : 0));
+        most = std::max(most, t);
+    }
+    return most;
+}
+
+static Plan plan(int T, int in, int vocab)
 {
     Plan p;
+    // Pairs take 7% less time a row where both halves of their 256-row tiles are full (2048 x
+    // 7168 over 163,840 ids: 15.4 against 16.4 ms for loss and gradient); 576 rows, 2.5 of
+    // their tiles, take 18% more.
+    p.cg = 100LL * ceil_div(T, 2 * BM) * 2 < 107LL * ceil_div(T, BM) ? 2 : 1;
     p.Tpad = ceil_div(T, ROW_PAD) * ROW_PAD;
     p.tiles = ceil_div(vocab, BN);
-    // a piece's dz takes about 64 MB, at least eight tiles
-    const long long tiles = std::max<long long>(8, (64LL << 20) / ((long long)p.Tpad * 2 * BN));
+    // a piece's dz takes about 128 MB, at least eight tiles
+    const long long tiles = std::max<long long>(8, (128LL << 20) / ((long long)p.Tpad * 2 * BN));
     p.piece = (int)std::min<long long>(tiles, p.tiles) * BN;
-    p.ldz = p.piece;
+    p.pieces = ceil_div(vocab, p.piece);
+    p.dz_bytes = (size_t)p.Tpad * p.piece * 2;
+    // dX has few tiles with long sums over the ids: split them where that shortens the busiest
+    // worker of the launches (148 SMs), each unit's fp32 sums costing about 16 steps to write
+    // and read back
+    const int rows = ceil_div(T, BM * p.cg), cols = ceil_div(in, BN), steps = p.piece / KB, workers = 148 / p.cg;
+    const long long n_w = (long long)ceil_div(p.piece, BM * p.cg) * cols, n_z = (long long)rows * (p.piece / BN);
+    double best = 0.0;
+    p.splits = 1;
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (s > 1 && steps / s < 4) break;
+        const int len = ceil_div(steps, s);
+        const double cost[3] = {len + (s > 1 || p.pieces > 1 ? 16.0 : 4.0), ceil_div(T, KB) + 4.0, ceil_div(in, KB) + 4.0};
+        const double t = busiest({(long long)rows * cols * s, n_w, 0}, cost, workers) +
+                         (p.pieces - 1) * busiest({(long long)rows * cols * s, n_w, n_z}, cost, workers);
+        if (s == 1 || t < 0.98 * best) {
+            best = t;
+            p.splits = s;
+        }
+    }
+    p.split_steps = ceil_div(steps, p.splits);
+    p.splits = ceil_div(steps, p.split_steps);
     return p;
 }
 
 struct Ws {
-    int *n_live, *place, *row_of, *ids, *count;
+    int *n_live, *row_of, *ids, *count;
     float *mass, *entropy, *zt, *acc;
     float2 *part;
-    __nv_bfloat16 *xp, *dz;
+    __nv_bfloat16 *xp, *dz[2];
 };
 
 // K = 0: cross entropy
@@ -694,7 +939,6 @@ static size_t layout(Ws *w, char *base, const Plan &p, int T, int in, int K, boo
     };
     Ws x{};
     x.n_live = (int *)take(4);
-    x.place = (int *)take((size_t)T * 4);
     x.row_of = (int *)take((size_t)T * 4);
     x.xp = (__nv_bfloat16 *)take((size_t)p.Tpad * in * 2);
     if (K) {
@@ -707,8 +951,9 @@ static size_t layout(Ws *w, char *base, const Plan &p, int T, int in, int K, boo
         x.part = (float2 *)take((size_t)p.tiles * 2 * p.Tpad * 8);
         x.zt = (float *)take((size_t)T * (K ? K : 1) * 4);
     } else {
-        x.dz = (__nv_bfloat16 *)take((size_t)p.Tpad * p.ldz * 2);
-        if (p.piece < p.tiles * BN) x.acc = (float *)take((size_t)p.Tpad * in * 4);
+        x.dz[0] = (__nv_bfloat16 *)take(p.dz_bytes);
+        x.dz[1] = p.pieces > 1 ? (__nv_bfloat16 *)take(p.dz_bytes) : x.dz[0];
+        if (p.pieces > 1 || p.splits > 1) x.acc = (float *)take((size_t)p.splits * p.Tpad * in * 4);
     }
     if (w) *w = x;
     return o;
@@ -728,8 +973,8 @@ static int prepare_device(int *sms)
     static std::atomic<uint64_t> ready{0};          // devices whose kernels have their shared memory
     const uint64_t bit = 1ull << (dev & 63);
     if (dev < 64 && (ready.load() & bit)) return K3GPU_OK;
-    for (const void *f : {(const void *)head_kernel<LOSS>, (const void *)head_kernel<DZ>,
-                          (const void *)head_kernel<GRADS>})
+    for (const void *f : {(const void *)head_kernel<LOSS, 1>, (const void *)head_kernel<GRAD, 1>,
+                          (const void *)head_kernel<GRAD, 2>})
         if ((st = cuda_status(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)))) return st;
     if (dev < 64) ready.fetch_or(bit);
     return K3GPU_OK;
@@ -748,7 +993,7 @@ struct Call {
 
 // The targets, the rows that count and their hidden states; fills the common arguments.
 static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w, float *loss, float *lse,
-                  uint16_t *dX, int lddx)
+                  uint16_t *dX, int lddx, int cg)
 {
     int st;
     if (c.K) {
@@ -756,85 +1001,118 @@ static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w
                                               1.0f / c.temp);
         if ((st = launch_status())) return st;
     }
-    plan_kernel<<<1, 1024, 0, c.s>>>(w.place, w.row_of, w.n_live, c.K ? nullptr : c.label, w.count, c.T, c.vocab);
-    if ((st = launch_status())) return st;
-    const int direct_ok = c.ldx % 8 == 0 && aligned(c.X, 16);
-    gather_kernel<<<c.T + ROW_PAD, 256, 0, c.s>>>(w.xp, loss, lse, reinterpret_cast<__nv_bfloat16 *>(dX), lddx, c.X,
-                                                  c.ldx, w.place, w.n_live, c.T, c.in, p.Tpad, direct_ok);
+    const int in_place = c.ldx % 8 == 0 && aligned(c.X, 16);
+    const int rows = std::max(8, ceil_div(c.T, PACK_BLOCKS));
+    pack_kernel<<<ceil_div(c.T, rows), 256, 0, c.s>>>(w.row_of, w.n_live, w.xp, loss, lse,
+                                                      reinterpret_cast<__nv_bfloat16 *>(dX), lddx, c.X, c.ldx,
+                                                      in_place, c.K ? nullptr : c.label, w.count, c.T, c.in, c.vocab,
+                                                      rows);
     if ((st = launch_status())) return st;
     *a = Args{};
-    a->T = c.T; a->in = c.in; a->vocab = c.vocab;
+    a->T = c.T; a->in = c.in;
     a->n_live = w.n_live; a->row_of = w.row_of; a->Tpad = p.Tpad;
+    a->x_in_place = in_place;
+    // the hidden states of a group stay in L2 while the vocabulary streams by: 48 MB of them
+    a->group_z = (int)std::max<long long>(ROW_PAD, std::min<long long>(MAX_T, (48LL << 20) / (c.in * 2LL)));
     a->ids = c.K ? w.ids : c.label;
     a->mass = w.mass; a->count = w.count;
     a->K = c.K ? c.K : 1;
     a->inv_temp = c.K ? 1.0f / c.temp : 1.0f;
     a->c = c.K ? (float)(1.4426950408889634 / (double)c.temp) : LOG2E;
-    a->x_direct_ok = direct_ok;
-    // the group's hidden states take at most about 32 MB
-    a->group = std::max(1, std::min(64, (int)((32LL << 20) / ((long long)BM * c.in * 2))));
-    const void *x = direct_ok ? (const void *)c.X : (const void *)w.xp;
-    const long long ldx = direct_ok ? c.ldx : c.in, xr = direct_ok ? c.T : p.Tpad;
+    const void *x = in_place ? (const void *)c.X : (const void *)w.xp;
+    const long long ldx = in_place ? c.ldx : c.in, xr = in_place ? c.T : p.Tpad;
     if ((st = map2d(&maps->x_k, x, c.in, ldx, xr, BM))) return st;
     if ((st = map2d(&maps->x_mn, x, c.in, ldx, xr, 64))) return st;
     if ((st = map2d(&maps->xp_k, w.xp, c.in, c.in, p.Tpad, BM))) return st;
     if ((st = map2d(&maps->xp_mn, w.xp, c.in, c.in, p.Tpad, 64))) return st;
-    if ((st = map2d(&maps->w_k, c.W, c.in, c.in, c.vocab, BN))) return st;
+    if ((st = map2d(&maps->w_k, c.W, c.in, c.in, c.vocab, BN / cg))) return st;
     return map2d(&maps->w_mn, c.W, c.in, c.in, c.vocab, 64);
+}
+
+template <int MODE, int CG>
+static int launch_head(const Maps &maps, const Args &a, int sms, cudaStream_t s)
+{
+    if (CG == 1) {
+        head_kernel<MODE, CG><<<sms, THREADS, SMEM, s>>>(maps, a);
+        return launch_status();
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = CG;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(sms / CG * CG);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, head_kernel<MODE, CG>, maps, a);
+    const int st = launch_status();
+    return e != cudaSuccess ? cuda_status(e) : st;
 }
 
 static int forward(float *loss, float *lse, const Call &c, void *ws)
 {
     int sms = 0, st = prepare_device(&sms);
     if (st) return st;
-    const Plan p = plan(c.T, c.vocab);
+    const Plan p = plan(c.T, c.in, c.vocab);
     Ws w;
     layout(&w, static_cast<char *>(ws), p, c.T, c.in, c.K, false);
     Args a;
     Maps maps{};
-    if ((st = set_up(&a, &maps, c, p, w, loss, lse, nullptr, 0))) return st;
+    if ((st = set_up(&a, &maps, c, p, w, loss, lse, nullptr, 0, 1))) return st;
     a.part = w.part; a.zt = w.zt;
-    a.v0 = 0; a.vc = c.vocab;
-    head_kernel<LOSS><<<sms, THREADS, SMEM, c.s>>>(maps, a);
-    if ((st = launch_status())) return st;
+    a.z = Piece{0, c.vocab, nullptr};
+    if ((st = launch_head<LOSS, 1>(maps, a, sms, c.s))) return st;
     join_kernel<<<p.Tpad / 32, 1024, 0, c.s>>>(loss, lse, w.part, 2 * p.tiles, p.Tpad, w.row_of, w.n_live, w.zt, w.mass,
                                                w.count, w.entropy, a.K, a.inv_temp);
     return launch_status();
 }
 
+// Launch i forms piece i's dz beside the dX and dW of piece i - 1 (two dz buffers), so each
+// launch has both kinds of units to fill the SMs with.
 static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const float *lse, const Call &c, void *ws)
 {
     int sms = 0, st = prepare_device(&sms);
     if (st) return st;
-    const Plan p = plan(c.T, c.vocab);
+    const Plan p = plan(c.T, c.in, c.vocab);
     Ws w;
     layout(&w, static_cast<char *>(ws), p, c.T, c.in, c.K, true);
     Args a;
     Maps maps{};
-    if ((st = set_up(&a, &maps, c, p, w, nullptr, nullptr, dX, lddx))) return st;
+    if ((st = set_up(&a, &maps, c, p, w, nullptr, nullptr, dX, lddx, p.cg))) return st;
     a.lse = lse; a.g = g;
-    a.dz = w.dz; a.ldz = p.ldz; a.acc = w.acc;
+    a.ldz = p.piece; a.acc = w.acc;
+    a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);
     a.dW = reinterpret_cast<__nv_bfloat16 *>(dW);
     a.want_dx = dX != nullptr; a.want_dw = dW != nullptr;
     a.lddx = lddx; a.vec_dx = lddx % 8 == 0 && aligned(dX, 16);
-    for (int v0 = 0; v0 < c.vocab; v0 += p.piece) {
-        a.v0 = v0;
-        a.vc = std::min(p.piece, c.vocab - v0);
-        a.first = v0 == 0; a.last = v0 + p.piece >= c.vocab;
-        if ((st = map2d(&maps.dz_k, w.dz, a.vc, p.ldz, p.Tpad, BM))) return st;
-        if ((st = map2d(&maps.dz_mn, w.dz, a.vc, p.ldz, p.Tpad, 64))) return st;
-        head_kernel<DZ><<<sms, THREADS, SMEM, c.s>>>(maps, a);
-        if ((st = launch_status())) return st;
-        head_kernel<GRADS><<<sms, THREADS, SMEM, c.s>>>(maps, a);
-        if ((st = launch_status())) return st;
+    a.z_before_dw = c.in > c.T;
+    for (int i = 0; i <= p.pieces; i++) {
+        a.d = a.z;
+        a.first = i == 1; a.last = i == p.pieces;
+        const int v0 = i * p.piece;
+        a.z = i < p.pieces ? Piece{v0, std::min(p.piece, c.vocab - v0), w.dz[i & 1]} : Piece{};
+        if (i > 0) {
+            if ((st = map2d(&maps.dz_k, a.d.dz, a.d.vc, p.piece, p.Tpad, BM))) return st;
+            if ((st = map2d(&maps.dz_mn, a.d.dz, a.d.vc, p.piece, p.Tpad, 64))) return st;
+        }
+        st = p.cg == 1 ? launch_head<GRAD, 1>(maps, a, sms, c.s) : launch_head<GRAD, 2>(maps, a, sms, c.s);
+        if (st) return st;
+    }
+    if (dX && p.splits > 1) {
+        sum_splits_kernel<<<dim3(ceil_div(c.in, 1024), c.T), 128, 0, c.s>>>(a.dX, lddx, a.vec_dx, w.acc, p.splits, p.Tpad,
+                                                                            c.in, w.row_of, w.n_live);
+        return launch_status();
     }
     return K3GPU_OK;
 }
 
 static size_t workspace_bytes(int T, int in, int vocab, int K)
 {
-    const Plan p = plan(T, vocab);
+    const Plan p = plan(T, in, vocab);
     return std::max(layout(nullptr, nullptr, p, T, in, K, false), layout(nullptr, nullptr, p, T, in, K, true));
 }
 
