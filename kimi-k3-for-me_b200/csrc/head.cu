@@ -53,7 +53,8 @@ constexpr int BM = 128, BN = 256, KB = 64; // rows a CTA, columns a unit
 constexpr int NU = 4;                      // units published ahead
 constexpr int A_BYTES = BM * KB * 2;
 constexpr int RING = 192 * 1024;           // the stages: 4 of 48 KB, or 6 of 32 KB in a pair
-constexpr int SMEM = RING + 512;
+constexpr int OUT_BYTES = 32 * 64 * 2;     // a warp's 32 rows x 64 columns on their way out
+constexpr int SMEM = RING + 8 * OUT_BYTES + 512;
 template <int CG> struct Stage {
     static constexpr int B_COLS = BN / CG, BYTES = A_BYTES + B_COLS * KB * 2, N = RING / BYTES;
 };
@@ -68,7 +69,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 enum Mode { LOSS, GRAD };
 enum Kind { Z, DX, DW };                   // what a unit of work forms
 
-// A vocabulary piece of the backward: ids v0 .. v0 + vc - 1, their dz [Tpad][ldz].
+// A vocabulary piece of the backward: ids v0 .. v0 + vc - 1, their dz [Tpad][piece].
 struct Piece {
     int v0, vc;
     __nv_bfloat16 *dz;
@@ -93,12 +94,11 @@ struct Args {
     // GRAD
     const float *lse, *g;       // by row; g may be nullptr (1)
     float inv_temp;
-    int ldz;
     Piece d;                    // vc = 0: no dX and dW units in this launch
     int want_dx, want_dw, first, last;
     int splits, split_steps;    // dX: K splits, 64-K steps of each
-    float *acc;                 // [splits][Tpad][in] dX before its last sum
-    __nv_bfloat16 *dX, *dW;
+    float4 *acc;                // dX before its last sum: by split, 128 x 256 tile, warp, 4 columns, lane
+    __nv_bfloat16 *dX;
     int lddx, vec_dx;
     int z_before_dw;            // the longer units come first
     int group_z;                // rows of z walked together
@@ -109,6 +109,7 @@ struct Maps {
     CUtensorMap w_k;            // W, K-major boxes (64 x a CTA's columns)
     CUtensorMap x_mn, xp_mn, w_mn;   // 64 x 64 boxes of rows as K
     CUtensorMap dz_k, dz_mn;    // piece d's dz, 64 x BM and 64 x 64 boxes
+    CUtensorMap z_out, w_out;   // piece z's dz and dW to write, 64 x 32 boxes
 };
 
 // A unit: a 128 CG x 256 tile of one product (or of one K split of it), worked on by a CTA
@@ -257,6 +258,34 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 64 columns of a warp's 32 rows, lane = row, from registers to an output: through shared
+// memory in the 128-byte swizzle and one TMA store. Lanes storing 16 bytes each to 32 rows
+// took 13,000 clocks a 128 x 256 unit; this takes a tenth. `off`: nothing is written.
+__device__ __forceinline__ void out_wait()
+{
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+template <typename F>
+__device__ __forceinline__ void store64(uint32_t buf, const CUtensorMap *m, int x, int y, bool off, int lane, F &&word8)
+{
+    if (lane == 0) out_wait();             // the buffer's last store has read it
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint4 o = word8(j);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) * 16))),
+                     "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w)
+                     : "memory");
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0 && !off) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(m), "r"(x),
+                     "r"(y), "r"(buf)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -321,8 +350,9 @@ __device__ __forceinline__ void loss_epilogue(const Args &a, float (&z)[HALF], R
     if (live) a.part[(size_t)(col0 / HALF) * a.Tpad + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
-__device__ __forceinline__ void dz_epilogue(const Args &a, float (&z)[HALF], RowTargets &tg, int t, int row,
-                                            bool live, int col0, float l2, float gt)
+__device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *out, uint32_t buf, float (&z)[HALF],
+                                            RowTargets &tg, int t, int row0, int lane, bool live, int col0, float l2,
+                                            float gt)
 {
 #pragma unroll
     for (int j = 0; j < HALF; j++) z[j] = ex2(fmaf(z[j], a.c, -l2));
@@ -337,14 +367,32 @@ __device__ __forceinline__ void dz_epilogue(const Args &a, float (&z)[HALF], Row
             tg.step(a);
         }
     // rows of the tile past the live ones are zeros: dW sums over them
-    uint4 *dst = reinterpret_cast<uint4 *>(a.z.dz + (size_t)row * a.ldz + col0);
+    const float gz = live ? gt : 0.0f;
 #pragma unroll
-    for (int j = 0; j < HALF; j += 8) {
-        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-        if (live)
-            o = make_uint4(pack_bf16(z[j] * gt, z[j + 1] * gt), pack_bf16(z[j + 2] * gt, z[j + 3] * gt),
-                           pack_bf16(z[j + 4] * gt, z[j + 5] * gt), pack_bf16(z[j + 6] * gt, z[j + 7] * gt));
-        dst[j / 8] = o;
+    for (int c0 = 0; c0 < HALF; c0 += 64)
+        store64(buf, out, col0 + c0, row0, false, lane, [&](int j) {
+            const float *f = z + c0 + 8 * j;
+            if (!live) return make_uint4(0u, 0u, 0u, 0u);
+            return make_uint4(pack_bf16(f[0] * gz, f[1] * gz), pack_bf16(f[2] * gz, f[3] * gz),
+                              pack_bf16(f[4] * gz, f[5] * gz), pack_bf16(f[6] * gz, f[7] * gz));
+        });
+}
+
+// where a warp's part of a dX tile lies in acc (float4s; its lanes follow)
+__device__ __forceinline__ size_t acc_at(const Args &a, int split, int row0, int col0, int w)
+{
+    const size_t tile = ((size_t)split * (a.Tpad / BM) + row0 / BM) * ((a.in + BN - 1) / BN) + col0 / BN;
+    return (tile * 8 + w) * (HALF / 4) * 32;
+}
+__device__ __forceinline__ void put8(__nv_bfloat16 *out, const float4 &f0, const float4 &f1, bool vec)
+{
+    const uint4 o = make_uint4(pack_bf16(f0.x, f0.y), pack_bf16(f0.z, f0.w), pack_bf16(f1.x, f1.y), pack_bf16(f1.z, f1.w));
+    if (vec) {
+        *reinterpret_cast<uint4 *>(out) = o;
+    } else {
+        uint16_t *u = reinterpret_cast<uint16_t *>(out);
+        u[0] = (uint16_t)o.x; u[1] = (uint16_t)(o.x >> 16); u[2] = (uint16_t)o.y; u[3] = (uint16_t)(o.y >> 16);
+        u[4] = (uint16_t)o.z; u[5] = (uint16_t)(o.z >> 16); u[6] = (uint16_t)o.w; u[7] = (uint16_t)(o.w >> 16);
     }
 }
 
@@ -354,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
     using St = Stage<CG>;
     constexpr int NS = St::N;
     extern __shared__ __align__(1024) unsigned char smem[];
-    uint64_t *b_full = reinterpret_cast<uint64_t *>(smem + RING), *b_empty = b_full + NS;
+    uint64_t *b_full = reinterpret_cast<uint64_t *>(smem + RING + 8 * OUT_BYTES), *b_empty = b_full + NS;
     uint64_t *b_done = b_empty + NS, *b_free = b_done + 2, *b_unit = b_free + 2, *b_took = b_unit + NU;
     int4 *unit_slot = reinterpret_cast<int4 *>(b_took + NU);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(unit_slot + NU);
@@ -479,6 +527,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const uint32_t buf = s_addr(smem + RING + (warp - 2) * OUT_BYTES);
         int use = 0;
         // the next finished accumulator
         auto finished = [&]() {
@@ -506,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
             __syncwarp();
             if (lane == 0) bar_arrive(s_addr(&b_took[slot]));
             if (t.kind < 0) break;
-            const int row = t.m0 + rank * BM + q * 32 + lane;   // packed row (z, dX) or id of the piece (dW)
+            const int row0 = t.m0 + rank * BM + q * 32, row = row0 + lane;   // packed row (z, dX), id of the piece (dW)
             const int col0 = t.n0 + half * HALF;
             const uint32_t src = tmem + lanes + (uint32_t)(half * HALF);
             if (MODE == LOSS || t.kind == Z) {
@@ -541,50 +590,63 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 }
                 if (failed) break;
                 if (MODE == LOSS) loss_epilogue(a, z, tg, tr, row, live, col0);
-                else dz_epilogue(a, z, tg, tr, row, live, col0, l2, gt);
+                else dz_epilogue(a, &maps.z_out, buf, z, tg, tr, row0, lane, live, col0, l2, gt);
                 __syncwarp();
+            } else if (t.kind == DW) {
+                if (t.steps > 0 && !finished()) { failed = true; break; }
+                for (int c0 = 0; c0 < HALF; c0 += 64) {
+                    uint32_t v[2][32];
+                    if (t.steps > 0) {
+                        tmem_ld32(src + (uint32_t)((use & 1) * BN + c0), v[0]);
+                        tmem_ld32(src + (uint32_t)((use & 1) * BN + c0 + 32), v[1]);
+                        tmem_wait_ld();
+                        if (c0 + 64 == HALF) release();
+                    } else {               // no row counts
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[0][j] = v[1][j] = 0u;
+                    }
+                    const int col = col0 + c0;
+                    store64(buf, &maps.w_out, col, a.d.v0 + row0, col >= a.in || row0 >= a.d.vc, lane, [&](int j) {
+                        const uint32_t *f = v[j >> 2] + 8 * (j & 3);
+                        auto pk = [&](int k) { return pack_bf16(__uint_as_float(f[k]), __uint_as_float(f[k + 1])); };
+                        return make_uint4(pk(0), pk(2), pk(4), pk(6));
+                    });
+                }
             } else {
-                const bool dx = t.kind == DX;
-                const bool live = dx ? row < n_live : row < a.d.vc;
-                const bool sum = dx && (a.splits > 1 || !a.last), add = dx && !a.first;
-                float *acc = a.acc + ((size_t)t.split * a.Tpad + row) * a.in;
-                __nv_bfloat16 *out = nullptr;
-                if (live) out = dx ? a.dX + (size_t)a.row_of[row] * a.lddx : a.dW + (size_t)(a.d.v0 + row) * a.in;
-                const bool vec = dx ? a.vec_dx : 1;
+                const bool live = row < n_live;
+                const bool sum = a.splits > 1 || !a.last, add = !a.first;
+                float4 *acc = a.acc + acc_at(a, t.split, t.m0 + rank * BM, t.n0, warp - 2) + lane;
+                __nv_bfloat16 *out = live ? a.dX + (size_t)a.row_of[row] * a.lddx : nullptr;
                 if (t.steps > 0 && !finished()) { failed = true; break; }
                 for (int c0 = 0; c0 < HALF; c0 += 32) {
-                    const int col = col0 + c0;
                     uint32_t v[32];
                     __syncwarp();
                     if (t.steps > 0) {
                         tmem_ld32(src + (uint32_t)((use & 1) * BN + c0), v);
                         tmem_wait_ld();
-                    } else {
+                    } else {               // a split past a short last piece
 #pragma unroll
                         for (int j = 0; j < 32; j++) v[j] = 0u;
                     }
+                    if (!live) continue;
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {      // `in` is a multiple of 8
-                        if (!live || col + j >= a.in) continue;
-                        float f[8];
-#pragma unroll
-                        for (int u = 0; u < 8; u++) f[u] = __uint_as_float(v[j + u]);
+                        float4 f0, f1;
+                        f0 = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]),
+                                         __uint_as_float(v[j + 3]));
+                        f1 = make_float4(__uint_as_float(v[j + 4]), __uint_as_float(v[j + 5]),
+                                         __uint_as_float(v[j + 6]), __uint_as_float(v[j + 7]));
+                        const int at = (c0 + j) / 4 * 32;
                         if (add) {
-                            const float4 p0 = *reinterpret_cast<const float4 *>(acc + col + j);
-                            const float4 p1 = *reinterpret_cast<const float4 *>(acc + col + j + 4);
-                            f[0] += p0.x; f[1] += p0.y; f[2] += p0.z; f[3] += p0.w;
-                            f[4] += p1.x; f[5] += p1.y; f[6] += p1.z; f[7] += p1.w;
+                            const float4 p0 = acc[at], p1 = acc[at + 32];
+                            f0.x += p0.x; f0.y += p0.y; f0.z += p0.z; f0.w += p0.w;
+                            f1.x += p1.x; f1.y += p1.y; f1.z += p1.z; f1.w += p1.w;
                         }
                         if (sum) {
-                            *reinterpret_cast<float4 *>(acc + col + j) = make_float4(f[0], f[1], f[2], f[3]);
-                            *reinterpret_cast<float4 *>(acc + col + j + 4) = make_float4(f[4], f[5], f[6], f[7]);
-                        } else if (vec) {
-                            *reinterpret_cast<uint4 *>(out + col + j) =
-                                make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
-                                           pack_bf16(f[6], f[7]));
-                        } else {
-#pragma unroll
-                            for (int u = 0; u < 8; u++) out[col + j + u] = __float2bfloat16_rn(f[u]);
+                            acc[at] = f0;
+                            acc[at + 32] = f1;
+                        } else if (col0 + c0 + j < a.in) {
+                            put8(out + col0 + c0 + j, f0, f1, a.vec_dx);
                         }
                     }
                 }
@@ -592,6 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 if (t.steps > 0) release();
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (failed && lane == 0) flag(DEV_TIMEOUT);
     }
     fence_before();
@@ -606,28 +669,24 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
     }
 }
 
-// dX = the splits' sums in order, as bf16: block (x, y) 8 columns a thread of packed row y
-__global__ void __launch_bounds__(128) sum_splits_kernel(__nv_bfloat16 *__restrict__ dX, int lddx, int vec,
-                                                         const float *__restrict__ acc, int splits, int Tpad, int in,
-                                                         const int *__restrict__ row_of, const int *__restrict__ n_live)
+// dX = the splits' sums in order, as bf16. Block (tile, p): columns 8 p .. and 128 + 8 p .. of a
+// 128 x 256 tile, a warp per epilogue warp's part.
+__global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
 {
-    const int row = blockIdx.y, col = (blockIdx.x * 128 + threadIdx.x) * 8;
-    if (row >= *n_live || col >= in) return;
-    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = 0; s < splits; s++) {
-        const float4 *p = reinterpret_cast<const float4 *>(acc + ((size_t)s * Tpad + row) * in + col);
-        const float4 p0 = p[0], p1 = p[1];
-        f[0] += p0.x; f[1] += p0.y; f[2] += p0.z; f[3] += p0.w;
-        f[4] += p1.x; f[5] += p1.y; f[6] += p1.z; f[7] += p1.w;
+    const int cols = (a.in + BN - 1) / BN, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row0 = (int)(blockIdx.x / cols) * BM, n0 = (int)(blockIdx.x % cols) * BN;
+    const int row = row0 + ((w + 2) & 3) * 32 + lane, col = n0 + (w >> 2) * HALF + (int)blockIdx.y * 8;
+    if (row >= *a.n_live || col >= a.in) return;
+    float4 f0 = make_float4(0, 0, 0, 0), f1 = f0;
+    const float4 *p = a.acc + acc_at(a, 0, row0, n0, w) + (int)blockIdx.y * 64 + lane;
+    const size_t step = acc_at(a, 1, 0, 0, 0);
+#pragma unroll 4
+    for (int s = 0; s < a.splits; s++, p += step) {
+        const float4 p0 = p[0], p1 = p[32];
+        f0.x += p0.x; f0.y += p0.y; f0.z += p0.z; f0.w += p0.w;
+        f1.x += p1.x; f1.y += p1.y; f1.z += p1.z; f1.w += p1.w;
     }
-    __nv_bfloat16 *out = dX + (size_t)row_of[row] * lddx + col;
-    if (vec) {
-        *reinterpret_cast<uint4 *>(out) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]),
-                                                     pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-    } else {
-#pragma unroll
-        for (int u = 0; u < 8; u++) out[u] = __float2bfloat16_rn(f[u]);
-    }
+    put8(a.dX + (size_t)a.row_of[row] * a.lddx + col, f0, f1, a.vec_dx);
 }
 
 // One block per row: the row's teacher entries as masses over ids in ascending order.
@@ -923,7 +982,8 @@ static Plan plan(int T, int in, int vocab)
 
 struct Ws {
     int *n_live, *row_of, *ids, *count;
-    float *mass, *entropy, *zt, *acc;
+    float *mass, *entropy, *zt;
+    float4 *acc;
     float2 *part;
     __nv_bfloat16 *xp, *dz[2];
 };
@@ -953,7 +1013,7 @@ static size_t layout(Ws *w, char *base, const Plan &p, int T, int in, int K, boo
     } else {
         x.dz[0] = (__nv_bfloat16 *)take(p.dz_bytes);
         x.dz[1] = p.pieces > 1 ? (__nv_bfloat16 *)take(p.dz_bytes) : x.dz[0];
-        if (p.pieces > 1 || p.splits > 1) x.acc = (float *)take((size_t)p.splits * p.Tpad * in * 4);
+        if (p.pieces > 1 || p.splits > 1) x.acc = (float4 *)take((size_t)p.splits * p.Tpad * ceil_div(in, BN) * BN * 4);
     }
     if (w) *w = x;
     return o;
@@ -1083,18 +1143,19 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     Maps maps{};
     if ((st = set_up(&a, &maps, c, p, w, nullptr, nullptr, dX, lddx, p.cg))) return st;
     a.lse = lse; a.g = g;
-    a.ldz = p.piece; a.acc = w.acc;
+    a.acc = w.acc;
     a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);
-    a.dW = reinterpret_cast<__nv_bfloat16 *>(dW);
     a.want_dx = dX != nullptr; a.want_dw = dW != nullptr;
     a.lddx = lddx; a.vec_dx = lddx % 8 == 0 && aligned(dX, 16);
     a.z_before_dw = c.in > c.T;
+    if (dW && (st = map2d(&maps.w_out, dW, c.in, c.in, c.vocab, 32))) return st;
     for (int i = 0; i <= p.pieces; i++) {
         a.d = a.z;
         a.first = i == 1; a.last = i == p.pieces;
         const int v0 = i * p.piece;
         a.z = i < p.pieces ? Piece{v0, std::min(p.piece, c.vocab - v0), w.dz[i & 1]} : Piece{};
+        if (i < p.pieces && (st = map2d(&maps.z_out, a.z.dz, p.piece, p.piece, p.Tpad, 32))) return st;
         if (i > 0) {
             if ((st = map2d(&maps.dz_k, a.d.dz, a.d.vc, p.piece, p.Tpad, BM))) return st;
             if ((st = map2d(&maps.dz_mn, a.d.dz, a.d.vc, p.piece, p.Tpad, 64))) return st;
@@ -1103,8 +1164,7 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
         if (st) return st;
     }
     if (dX && p.splits > 1) {
-        sum_splits_kernel<<<dim3(ceil_div(c.in, 1024), c.T), 128, 0, c.s>>>(a.dX, lddx, a.vec_dx, w.acc, p.splits, p.Tpad,
-                                                                            c.in, w.row_of, w.n_live);
+        sum_splits_kernel<<<dim3(ceil_div(c.T, BM) * ceil_div(c.in, BN), HALF / 8), 256, 0, c.s>>>(a);
         return launch_status();
     }
     return K3GPU_OK;
