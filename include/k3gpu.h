@@ -401,8 +401,8 @@ int k3gpu_lm_head_argmax(int *arg, const float *X, int ldx, const uint16_t *W, i
  * val [rows][K] descending and idx [rows][K] their ids, equal values by ascending id; NaN
  * is never taken; a row with fewer than K values that are not NaN ends in idx -1, val
  * -inf. logits [rows][vocab], e.g. a verify sweep's (k3gpu_model_verify): the teacher
- * entries of k3gpu_lm_head_distill. 1 <= K <= 128, rows <= 65535. The workspace is 16-byte
- * aligned. */
+ * entries of k3gpu_lm_head_distill. 1 <= K <= 128, rows <= 65535, vocab <= 2^30. The
+ * workspace is 16-byte aligned. */
 size_t k3gpu_topk_logits_workspace(int rows, int vocab, int K);
 int k3gpu_topk_logits(int *idx, float *val, const float *logits, int rows, int vocab, int K,
                       void *workspace, size_t ws_bytes, void *stream);

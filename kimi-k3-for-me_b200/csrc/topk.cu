@@ -3,17 +3,20 @@
 //
 // Order: values descending, equal values by ascending id; NaN is never taken (argmax's
 // rule), -inf is taken after every finite value. Each value becomes a 32-bit key that
-// orders as the floats do (the sign folded in, -0 as +0, NaN as 0, below -inf's key).
+// orders as the floats do (the sign folded in, -0 as +0, NaN as 0, below -inf's key); key and
+// complemented id make a 64-bit rank, and no two ranks are equal.
 //
-// The row is read once. A block walks its segment of the row in tiles; a value joins the
-// block's candidate list when its key is above the K-th largest kept so far (strictly:
-// tiles ascend in id, so an equal value comes after K better ones), and a tile that makes
-// the list outgrow KEEP is followed by a selection that cuts it to K and raises the bar.
-// Random rows take a handful of selections a segment (the expected number of values above
-// a running K-th largest grows with the log of the length); an ascending row takes one per
-// tile and is still exact. A second kernel selects among the segments' lists and writes
-// the K in order, each value's place counted directly (K <= 128).
-// Bound by the read: K << vocab, about four instructions a value.
+// The row is read once, a block per segment of it, 8192 values a round, 32 a thread in
+// registers. The first round's bar: each warp's ceil(K / 8)-th largest of its lanes' maxima,
+// the least of the warps' (so at least K values reach it; of random values about 1% pass).
+// One comparison for four values; a quad with one above the bar is put aside whole in
+// shared memory, and after the round the block takes its values apart into the candidate
+// list, which is trimmed to about the K best by bisection on the ranks, raising the bar. Past
+// the first round the bar is strict: ids ascend, so an equal value comes behind K better ones.
+// A round with more such quads than fit (long runs of ascending values) is taken again in
+// small steps with a trim after each; the result is exact whatever the order.
+// A second kernel joins the segments' lists the same way and writes the K in order.
+// Bound by the read, about two instructions a value.
 #include <math.h>
 
 #include "common.cuh"
@@ -21,15 +24,20 @@
 namespace k3 {
 namespace topk {
 
-constexpr int THREADS = 512;
-constexpr int PER = 8;                       // values a thread holds of a tile
-constexpr int TILE = THREADS * PER;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int QUADS = 8;                     // float4s a thread holds of a round
+constexpr int ROUND = THREADS * QUADS * 4;
 constexpr int MAXK = 128;
-constexpr int KEEP = 1024;                   // candidates kept before a selection is due
-constexpr int CAP = KEEP + TILE;             // a tile can join whole
-constexpr int MAX_SEG = 32;                  // segments a row: their lists fit one selection
-constexpr int HOLD = (CAP + THREADS - 1) / THREADS;   // candidates a thread holds in a selection
-static_assert(MAX_SEG * MAXK <= CAP, "the merge holds every segment's list");
+constexpr int MORE = 64;                     // candidates past K before a trim is due
+constexpr int SLACK = 16;                    // a trim leaves at most K + SLACK
+constexpr int STEP = 1024;                   // values a step of a round taken again
+constexpr int ASIDE = 512;                   // quads a round puts aside
+constexpr int LIST = 2304;
+constexpr int HOLD = LIST / THREADS;         // candidates a thread holds in a trim
+constexpr int MAX_SEG = 32;
+constexpr int MERGE = MAX_SEG * MAXK / THREADS;   // candidates a thread holds in the merge
+static_assert(MAXK + MORE + 4 * ASIDE <= LIST && MAXK + MORE + STEP <= LIST, "what joins fits behind what is kept");
+static_assert(MAXK + MORE <= THREADS, "one candidate a thread in the last sort");
 
 __device__ __forceinline__ uint32_t key_of(float v)
 {
@@ -42,12 +50,16 @@ __device__ __forceinline__ float value_of(uint32_t k)
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
+__device__ __forceinline__ uint64_t rank_of(uint32_t key, int id) { return (uint64_t)key << 32 | (uint32_t)~id; }
+
 struct Shared {
-    uint32_t key[CAP];
-    int id[CAP];
-    int n;                          // candidates in the list
+    uint64_t rank[LIST];
+    float4 quad[ASIDE];
+    int quad_id[ASIDE];
+    int n, n_quads;                 // candidates; quads above the bar (those past ASIDE were dropped)
     uint32_t bar;                   // a value joins when its key is above this
-    int part[2][THREADS / 32];
+    int part[2][WARPS];
+    uint32_t low[WARPS];
 };
 
 // block-wide sum of a count, one barrier (the partial array alternates)
@@ -58,162 +70,239 @@ __device__ __forceinline__ int block_count(int c, int *part)
     __syncthreads();
     int t = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) t += part[w];
+    for (int w = 0; w < WARPS; w++) t += part[w];
     return t;
 }
 
-// Cut the list to its K best, in any order. Called by the whole block with the list and n
-// visible; leaves them, and the bar, visible. The K-th largest key is the largest t with at
-// least K keys >= t, found bit by bit; where its equals overflow the K places, the largest
-// id that still fits is found the same way.
-__device__ void select(Shared &s, int K)
+// A first bar from the threads' largest keys: at least K values have a key above it.
+__device__ __forceinline__ void first_bar(Shared &s, uint32_t most, int K)
 {
-    const int n = s.n;
-    if (n <= K) {
-        __syncthreads();
-        return;
-    }
-    uint32_t key[HOLD];
-    int id[HOLD];
-#pragma unroll
-    for (int i = 0; i < HOLD; i++) {
-        const int x = threadIdx.x + i * THREADS;
-        key[i] = x < n ? s.key[x] : 0u;
-        id[i] = x < n ? s.id[x] : 0x7fffffff;
-    }
+    const int need = (K + WARPS - 1) / WARPS;
     uint32_t t = 0;
-    int flip = 0, at_least = n;
+#pragma unroll
     for (int b = 31; b >= 0; b--) {
         const uint32_t mid = t | (1u << b);
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < HOLD; i++) c += key[i] >= mid;
-        c = block_count(c, s.part[flip ^= 1]);
-        if (c >= K) {
-            t = mid;
-            at_least = c;
-            if (c == K) break;
-        }
+        if (__popc(__ballot_sync(0xffffffffu, most >= mid)) >= need) t = mid;
     }
-    int last = 0x7fffffff;          // keys equal to t stay up to this id
-    if (at_least > K) {
-        int above = 0;
-#pragma unroll
-        for (int i = 0; i < HOLD; i++) above += key[i] > t;
-        above = block_count(above, s.part[flip ^= 1]);
-        // the smallest id with (K - above) equals at or below it
-        int lo = 0;
-        for (int b = 30; b >= 0; b--) {
-            const int mid = lo | (1 << b);
-            int c = 0;
-#pragma unroll
-            for (int i = 0; i < HOLD; i++) c += key[i] == t && id[i] < mid;
-            c = block_count(c, s.part[flip ^= 1]);
-            if (c < K - above) lo = mid;
-        }
-        last = lo;
-    }
-    __syncthreads();                // every thread holds its candidates: the list is rewritten
-    if (threadIdx.x == 0) s.n = 0;
+    if ((threadIdx.x & 31) == 0) s.low[threadIdx.x >> 5] = t;
     __syncthreads();
+    uint32_t low = s.low[0];
 #pragma unroll
-    for (int i = 0; i < HOLD; i++) {
-        const int x = threadIdx.x + i * THREADS;
-        if (x < n && (key[i] > t || (key[i] == t && id[i] <= last))) {
-            const int p = atomicAdd(&s.n, 1);
-            s.key[p] = key[i];
-            s.id[p] = id[i];
-        }
-    }
-    if (threadIdx.x == 0) s.bar = t;
+    for (int w = 1; w < WARPS; w++) low = min(low, s.low[w]);
+    // just below it; -0 has no key of its own, and as a float it is not below 0
+    if (threadIdx.x == 0) s.bar = low == 0x80000000u ? low - 2 : low ? low - 1 : 0u;
     __syncthreads();
 }
 
-// grid (segments, rows): the segment's K best to cand_key/cand_id [rows][segments][K], the
-// places past its candidates with key 0
-__global__ void __launch_bounds__(THREADS) segment_kernel(uint32_t *__restrict__ cand_key, int *__restrict__ cand_id,
-                                                          const float *__restrict__ logits, int vocab, int seg_len,
-                                                          int K)
+__device__ __forceinline__ void join(Shared &s, uint32_t key, int id, uint32_t bar)
 {
-    extern __shared__ __align__(16) unsigned char topk_dyn[];
-    Shared &s = *reinterpret_cast<Shared *>(topk_dyn);
+    if (key > bar) s.rank[atomicAdd(&s.n, 1)] = rank_of(key, id);
+}
+
+// Trim the list to between K and K + SLACK of its best and raise the bar to them. Called by
+// the whole block with n = s.n read by all; leaves the list, n and the bar visible; returns n.
+__device__ __noinline__ int trim(Shared &s, int n, int K)
+{
+    uint64_t r[HOLD];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < HOLD; i++) {
+        const int x = threadIdx.x + i * THREADS;
+        r[i] = x < n ? s.rank[x] : 0ull;
+        top = max(top, (uint32_t)(r[i] >> 32));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) s.low[threadIdx.x >> 5] = top;
+    uint64_t lo = (uint64_t)(s.bar + 1u) << 32;        // n ranks at or above it
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) top = max(top, s.low[w]);
+    uint64_t hi = (uint64_t)(top + 1u) << 32;          // none
+    int flip = 0;
+    while (hi - lo > 1) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < HOLD; i++) c += r[i] >= mid;
+        c = block_count(c, s.part[flip ^= 1]);
+        if (c >= K) {
+            lo = mid;
+            if (c <= K + SLACK) break;
+        } else {
+            hi = mid;
+        }
+    }
+    __syncthreads();                // every thread holds its candidates: the list is rewritten
+    if (threadIdx.x == 0) {
+        s.n = 0;
+        s.bar = (uint32_t)(lo >> 32);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HOLD; i++)
+        if (r[i] >= lo) s.rank[atomicAdd(&s.n, 1)] = r[i];
+    __syncthreads();
+    n = s.n;
+    __syncthreads();
+    return n;
+}
+
+// The list's K best in order, by counting each one's place; places past the list are 0.
+__device__ __forceinline__ void sort(Shared &s, int n, int K)
+{
+    if (n > K + MORE) n = trim(s, n, K);
+    if (n + threadIdx.x < (unsigned)((n + 3) & ~3)) s.rank[n + threadIdx.x] = 0;
+    __syncthreads();
+    const uint64_t r = (int)threadIdx.x < n ? s.rank[threadIdx.x] : 0;
+    int place = (int)threadIdx.x < n ? 0 : THREADS;
+#pragma unroll 2
+    for (int j = 0; j < n; j += 4) {
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(&s.rank[j]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(&s.rank[j + 2]);
+        place += (a.x > r) + (a.y > r) + (b.x > r) + (b.y > r);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x >= n && (int)threadIdx.x < K) s.rank[threadIdx.x] = 0;
+    if (place < K) s.rank[place] = r;
+    __syncthreads();
+}
+
+__device__ __forceinline__ void write_out(const Shared &s, int *idx, float *val, int K)
+{
+    for (int k = threadIdx.x; k < K; k += THREADS) {
+        const uint64_t r = s.rank[k];
+        idx[k] = r ? (int)~(uint32_t)r : -1;
+        val[k] = r ? value_of((uint32_t)(r >> 32)) : -INFINITY;
+    }
+}
+
+// grid (segments, rows): the segment's K best, in order, to cand [rows][segments][K] (0 past its
+// candidates), or, of a row that is one segment, to idx and val
+__global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restrict__ cand, int *__restrict__ idx,
+                                                             float *__restrict__ val, const float *__restrict__ logits,
+                                                             int vocab, int seg_len, int K)
+{
+    __shared__ __align__(16) Shared s;
     const float *row = logits + (size_t)blockIdx.y * vocab;
     const int begin = blockIdx.x * seg_len, end = min(vocab, begin + seg_len);
-    if (threadIdx.x == 0) { s.n = 0; s.bar = 0; }
-    float v[PER];
-    auto fetch = [&](int base) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int x = base + i * THREADS + (int)threadIdx.x;
-            v[i] = x < end ? __ldg(row + x) : NAN;
-        }
-    };
-    fetch(begin);
+    if (threadIdx.x == 0) { s.n = s.n_quads = 0; s.bar = 0; }
     __syncthreads();
-    for (int base = begin; base < end; base += TILE) {
-        uint32_t key[PER];
+    // quads lie on 16-byte boundaries; the first may start before the segment
+    const int skew = (int)((reinterpret_cast<uintptr_t>(row + begin) & 15u) / 4);
+    int n = 0;
+    for (int base = begin - skew; base < end; base += ROUND) {
+        float4 v[QUADS];
 #pragma unroll
-        for (int i = 0; i < PER; i++) key[i] = key_of(v[i]);
-        if (base + TILE < end) fetch(base + TILE);
+        for (int i = 0; i < QUADS; i++) {
+            const int x = base + (i * THREADS + (int)threadIdx.x) * 4;
+            if (x >= begin && x + 4 <= end) {
+                v[i] = __ldcs(reinterpret_cast<const float4 *>(row + x));
+            } else {
+                v[i].x = x >= begin && x < end ? row[x] : NAN;
+                v[i].y = x + 1 >= begin && x + 1 < end ? row[x + 1] : NAN;
+                v[i].z = x + 2 >= begin && x + 2 < end ? row[x + 2] : NAN;
+                v[i].w = x + 3 >= begin && x + 3 < end ? row[x + 3] : NAN;
+            }
+        }
+        // fmaxf passes over NaN
+        auto most = [](const float4 &q) { return fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)); };
+        if (base + skew == begin) {
+            float m = NAN;
+#pragma unroll
+            for (int i = 0; i < QUADS; i++) m = fmaxf(m, most(v[i]));
+            first_bar(s, key_of(m), K);
+        }
         const uint32_t bar = s.bar;
+        const float bar_f = value_of(bar);            // NaN for an open bar: every quad passes
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (key[i] > bar) {
-                const int p = atomicAdd(&s.n, 1);
-                s.key[p] = key[i];
-                s.id[p] = base + i * THREADS + (int)threadIdx.x;
+        for (int i = 0; i < QUADS; i++)
+            if (!(most(v[i]) <= bar_f)) {
+                const int p = atomicAdd(&s.n_quads, 1);
+                if (p < ASIDE) {
+                    s.quad[p] = v[i];
+                    s.quad_id[p] = base + (i * THREADS + (int)threadIdx.x) * 4;
+                }
             }
         __syncthreads();
-        if (s.n > KEEP || (base == begin && s.n > K)) select(s, K);
-        __syncthreads();
+        const int aside = s.n_quads;
+        if (aside == 0) {                              // (read by all before anyone adds to it:
+            __syncthreads();                           //  the loads of the next round come between)
+            continue;
+        }
+        if (aside <= ASIDE) {
+            for (int p = threadIdx.x; p < aside; p += THREADS) {
+                const float4 q = s.quad[p];
+                const int x = s.quad_id[p];
+                join(s, key_of(q.x), x, bar);
+                join(s, key_of(q.y), x + 1, bar);
+                join(s, key_of(q.z), x + 2, bar);
+                join(s, key_of(q.w), x + 3, bar);
+            }
+            __syncthreads();
+            n = s.n;
+            if (threadIdx.x == 0) s.n_quads = 0;
+            __syncthreads();
+            if (n > K + MORE) n = trim(s, n, K);
+        } else {                                       // again, in steps that fit
+            const int stop = min(base + ROUND, end);
+            for (int x0 = max(base, begin); x0 < stop; x0 += STEP) {
+                const uint32_t now = s.bar;
+                for (int x = x0 + (int)threadIdx.x; x < min(x0 + STEP, stop); x += THREADS)
+                    join(s, key_of(row[x]), x, now);
+                __syncthreads();
+                n = s.n;
+                if (threadIdx.x == 0) s.n_quads = 0;
+                __syncthreads();
+                if (n > K + MORE) n = trim(s, n, K);
+            }
+        }
     }
-    select(s, K);
-    const size_t out = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * K;
-    for (int k = threadIdx.x; k < K; k += THREADS) {
-        cand_key[out + k] = k < s.n ? s.key[k] : 0u;
-        cand_id[out + k] = k < s.n ? s.id[k] : 0x7fffffff;
+    sort(s, n, K);
+    if (gridDim.x == 1) {
+        write_out(s, idx + (size_t)blockIdx.y * K, val + (size_t)blockIdx.y * K, K);
+        return;
     }
+    cand += ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * K;
+    for (int k = threadIdx.x; k < K; k += THREADS) cand[k] = s.rank[k];
 }
 
 // grid (rows): the K best of the segments' lists, in order
 __global__ void __launch_bounds__(THREADS) merge_kernel(int *__restrict__ idx, float *__restrict__ val,
-                                                        const uint32_t *__restrict__ cand_key,
-                                                        const int *__restrict__ cand_id, int nseg, int K)
+                                                        const uint64_t *__restrict__ cand, int nseg, int K)
 {
-    extern __shared__ __align__(16) unsigned char topk_dyn[];
-    Shared &s = *reinterpret_cast<Shared *>(topk_dyn);
-    const size_t in = (size_t)blockIdx.x * nseg * K, out = (size_t)blockIdx.x * K;
+    __shared__ __align__(16) Shared s;
+    const int total = nseg * K;
+    cand += (size_t)blockIdx.x * total;
     if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    for (int x = threadIdx.x; x < nseg * K; x += THREADS) {
-        const uint32_t k = cand_key[in + x];
-        if (k) {
-            const int p = atomicAdd(&s.n, 1);
-            s.key[p] = k;
-            s.id[p] = cand_id[in + x];
-        }
+    uint64_t r[MERGE];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < MERGE; i++) {
+        const int x = threadIdx.x + i * THREADS;
+        r[i] = x < total ? cand[x] : 0ull;
+        most = max(most, (uint32_t)(r[i] >> 32));
     }
-    __syncthreads();
-    select(s, K);
-    const int n = s.n;
-    for (int k = threadIdx.x; k < K; k += THREADS) {
-        if (k < n) {
-            int place = 0;
-            for (int j = 0; j < n; j++)
-                place += s.key[j] > s.key[k] || (s.key[j] == s.key[k] && s.id[j] < s.id[k]);
-            idx[out + place] = s.id[k];
-            val[out + place] = value_of(s.key[k]);
-        } else {
-            idx[out + k] = -1;
-            val[out + k] = -INFINITY;
-        }
+    first_bar(s, most, K);
+    // a step of four candidates a thread at a time (MERGE steps fit the list only trimmed)
+    int n = 0;
+    for (int i0 = 0; i0 < MERGE && i0 * THREADS < total; i0 += 4) {
+        const uint32_t bar = s.bar;
+#pragma unroll
+        for (int i = 0; i < MERGE; i++)
+            if (i / 4 == i0 / 4 && (uint32_t)(r[i] >> 32) > bar) s.rank[atomicAdd(&s.n, 1)] = r[i];
+        __syncthreads();
+        n = s.n;
+        __syncthreads();
+        if (n > K + MORE) n = trim(s, n, K);
     }
+    sort(s, n, K);
+    write_out(s, idx + (size_t)blockIdx.x * K, val + (size_t)blockIdx.x * K, K);
 }
 
 static int segments(int rows, int vocab)
 {
-    // about four blocks an SM of 148, no segment shorter than two tiles
-    const int want = ceil_div(4 * 148, rows), most = ceil_div(vocab, 2 * TILE);
+    // about four blocks an SM of 148, no segment shorter than a round
+    const int want = ceil_div(4 * 148, rows), most = ceil_div(vocab, ROUND);
     return std::max(1, std::min(std::min(want, most), MAX_SEG));
 }
 
@@ -226,7 +315,7 @@ extern "C" size_t k3gpu_topk_logits_workspace(int rows, int vocab, int K)
 {
     using namespace k3::topk;
     if (rows <= 0 || vocab <= 0 || K <= 0 || K > MAXK) return 0;
-    return 2 * a256((size_t)rows * segments(rows, vocab) * K * 4);
+    return a256((size_t)rows * segments(rows, vocab) * K * 8);
 }
 
 extern "C" int k3gpu_topk_logits(int *idx, float *val, const float *logits, int rows, int vocab, int K,
@@ -234,16 +323,15 @@ extern "C" int k3gpu_topk_logits(int *idx, float *val, const float *logits, int 
 {
     using namespace k3::topk;
     if (!idx || !val || !logits || !workspace || rows <= 0 || vocab <= 0 || K <= 0 || K > MAXK) return K3GPU_EINVAL;
-    if (rows > 65535 || !k3::aligned(workspace, 16)) return K3GPU_EINVAL;
+    if (rows > 65535 || vocab > 1 << 30 || !k3::aligned(logits, 4) || !k3::aligned(workspace, 16)) return K3GPU_EINVAL;
     if (ws_bytes < k3gpu_topk_logits_workspace(rows, vocab, K)) return K3GPU_ECAPACITY;
     const int nseg = segments(rows, vocab);
     const int seg_len = k3::ceil_div(k3::ceil_div(vocab, nseg), 4) * 4;
-    uint32_t *ck = static_cast<uint32_t *>(workspace);
-    int *ci = reinterpret_cast<int *>(static_cast<char *>(workspace) + a256((size_t)rows * nseg * K * 4));
+    uint64_t *cand = static_cast<uint64_t *>(workspace);
     cudaStream_t s = k3::as_stream(stream);
-    segment_kernel<<<dim3(nseg, rows), THREADS, sizeof(Shared), s>>>(ck, ci, logits, vocab, seg_len, K);
-    int st = k3::launch_status();
-    if (st) return st;
-    merge_kernel<<<rows, THREADS, sizeof(Shared), s>>>(idx, val, ck, ci, nseg, K);
+    segment_kernel<<<dim3(nseg, rows), THREADS, 0, s>>>(cand, idx, val, logits, vocab, seg_len, K);
+    const int st = k3::launch_status();
+    if (st || nseg == 1) return st;
+    merge_kernel<<<rows, THREADS, 0, s>>>(idx, val, cand, nseg, K);
     return k3::launch_status();
 }

@@ -94,8 +94,8 @@ def test_workspace_sizes(m):
 
 
 @pytest.mark.parametrize("kw", [dict(idx=None), dict(val=None), dict(logits=None), dict(ws=None), dict(rows=0),
-                                dict(rows=65536), dict(vocab=0), dict(K=0), dict(K=129),
-                                dict(ws=C.c_void_p((1 << 20) + 4))])
+                                dict(rows=65536), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(K=0), dict(K=129),
+                                dict(ws=C.c_void_p((1 << 20) + 4)), dict(logits=C.c_void_p((1 << 20) + 2))])
 def test_topk_refuses(m, kw):
     a = dict(idx=P, val=P, logits=P, rows=2, vocab=10, K=3, ws=P, bytes=1 << 20)
     a.update(kw)
