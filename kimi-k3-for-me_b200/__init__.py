@@ -13,6 +13,7 @@ The directory name is not a Python identifier, so callers load it by path::
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -586,129 +587,145 @@ def lm_head_argmax(X, W, ws=None, stream=None):
 
 
 # ------------------------------------------------------- fitting a draft head ------
-def _on(device, *tensors):
-    """Every tensor (None skipped) on the one CUDA device."""
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise K3Error(f"expected every tensor on {device}, got one on {t.device}")
+def _on_device_of(fn):
+    """Run a wrapper whose first argument is a CUDA tensor with that tensor's device current."""
+    @functools.wraps(fn)
+    def call(x, *args, **kw):
+        if not x.is_cuda:
+            raise K3Error("expected a CUDA tensor")
+        if x.device.index == torch.cuda.current_device():
+            return fn(x, *args, **kw)
+        with torch.cuda.device(x.device):
+            return fn(x, *args, **kw)
+    return call
 
 
-def _head_args(X, W, ws, need):
-    """The checks the draft-head losses share; the workspace when the caller gave none."""
-    for name, t in (("X", X), ("W", W)):
-        if not t.is_cuda or t.dim() != 2 or t.element_size() != 2 or t.dtype == torch.float16:
-            raise K3Error(f"{name}: expected a 2-D CUDA tensor of bfloat16 (or its bits)")
-    if X.shape[1] != W.shape[1]:
-        raise K3Error(f"X {tuple(X.shape)} and W {tuple(W.shape)} differ in width")
-    if X.stride(1) != 1 or (X.shape[0] > 1 and X.stride(0) < X.shape[1]):
-        raise K3Error("X: expected rows of consecutive elements that do not overlap")
-    return ws if ws is not None else workspace(need, X.device)
-
-
-def _row_stride(X):
-    return X.stride(0) if X.shape[0] > 1 else X.shape[1]
-
-
-def _rows_of(name, t, shape, dtype):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
-        raise K3Error(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+def _arg(name, t, device, dtype, shape):
+    """Device pointer of a contiguous tensor, checked against what the call needs."""
+    if t.device != device or t.dtype != dtype or t.shape != shape:
+        raise K3Error(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on "
+                      f"{t.device}")
     return ptr(t)
 
 
+def _head_args(X, W):
+    """(X pointer, row stride, W pointer, width, vocab, T) of a draft-head loss, checked."""
+    for name, t in (("X", X), ("W", W)):
+        if t.dim() != 2 or t.dtype not in (torch.bfloat16, torch.int16, torch.uint16):
+            raise K3Error(f"{name}: expected a 2-D tensor of bfloat16 (or its bits), got {t.dtype} {tuple(t.shape)}")
+    (T, n), (vocab, m) = X.shape, W.shape
+    if n != m or X.device != W.device:
+        raise K3Error(f"X {tuple(X.shape)} on {X.device} and W {tuple(W.shape)} on {W.device} do not match")
+    ldx = X.stride(0) if T > 1 else n
+    if X.stride(1) != 1 or ldx < n:
+        raise K3Error("X: expected rows of consecutive elements that do not overlap")
+    return C.c_void_p(X.data_ptr()), ldx, ptr(W), n, vocab, T
+
+
+def _scratch(ws, need, device):
+    if ws is None:
+        ws = workspace(need, device)
+    elif ws.device != device or ws.dtype != torch.uint8:
+        raise K3Error(f"workspace: expected uint8 on {device}, got {ws.dtype} on {ws.device}")
+    return ptr(ws), ws.numel(), ws     # the tensor is kept until the call is enqueued
+
+
+def _stream_of(stream, device):
+    return C.c_void_p((stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream)
+
+
+@_on_device_of
 def topk_logits(logits, K, ws=None, stream=None):
     """The K largest logits of each row of logits [rows][vocab]: (ids int32, values fp32)
     [rows][K], descending, equal values by ascending id, NaN never taken; a row that runs out
     ends in id -1, -inf. The teacher entries of lm_head_distill."""
     if logits.dim() != 2 or logits.dtype != torch.float32:
-        raise K3Error("logits: expected fp32 [rows][vocab]")
-    rows, vocab = logits.shape
-    with torch.cuda.device(logits.device):
-        idx = torch.empty((rows, K), dtype=torch.int32, device=logits.device)
-        val = torch.empty((rows, K), dtype=torch.float32, device=logits.device)
-        if rows == 0:
-            return idx, val
-        ws = ws if ws is not None else workspace(lib.k3gpu_topk_logits_workspace(rows, vocab, K), logits.device)
-        _on(logits.device, ws)
-        check(lib.k3gpu_topk_logits(ptr(idx), ptr(val), ptr(logits), rows, vocab, K, ptr(ws), ws.numel(),
-                                    stream_ptr(stream)), "k3gpu_topk_logits")
+        raise K3Error(f"logits: expected fp32 [rows][vocab], got {logits.dtype} {tuple(logits.shape)}")
+    (rows, vocab), dev = logits.shape, logits.device
+    idx = torch.empty((rows, K), dtype=torch.int32, device=dev)
+    val = torch.empty((rows, K), dtype=torch.float32, device=dev)
+    if rows == 0:
+        return idx, val
+    wp, wn, ws = _scratch(ws, lib.k3gpu_topk_logits_workspace(rows, vocab, K), dev)
+    check(lib.k3gpu_topk_logits(ptr(idx), ptr(val), ptr(logits), rows, vocab, K, wp, wn, _stream_of(stream, dev)),
+          "k3gpu_topk_logits")
     return idx, val
 
 
+@_on_device_of
 def lm_head_xent(X, W, label, ws=None, stream=None):
     """Softmax cross entropy of the lm_head product X [T][in] . W^T (bf16, the logits never
     written) against label int32 [T]: (loss, lse) fp32 [T]. A negative label is a row without a
     target: loss, lse and gradient 0."""
-    T, vocab = X.shape[0], W.shape[0]
-    with torch.cuda.device(X.device):
-        loss = torch.empty(T, dtype=torch.float32, device=X.device)
-        lse = torch.empty(T, dtype=torch.float32, device=X.device)
-        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_xent_workspace(T, X.shape[1], vocab))
-        _on(X.device, W, label, ws)
-        lab = _rows_of("label", label, (T,), torch.int32)
-        if T == 0:
-            return loss, lse
-        check(lib.k3gpu_lm_head_xent(ptr(loss), ptr(lse), X.data_ptr(), _row_stride(X), ptr(W), lab, X.shape[1], vocab, T,
-                                     ptr(ws), ws.numel(), stream_ptr(stream)), "k3gpu_lm_head_xent")
+    xp, ldx, w, n, vocab, T = _head_args(X, W)
+    dev = X.device
+    lab = _arg("label", label, dev, torch.int32, (T,))
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    lse = torch.empty(T, dtype=torch.float32, device=dev)
+    if T == 0:
+        return loss, lse
+    wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
+    check(lib.k3gpu_lm_head_xent(ptr(loss), ptr(lse), xp, ldx, w, lab, n, vocab, T, wp, wn, _stream_of(stream, dev)),
+          "k3gpu_lm_head_xent")
     return loss, lse
 
 
-def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
-    """The gradient of lm_head_xent from its lse and the loss's incoming gradient g fp32 [T]
-    (None: 1): (dX [T][in], dW [vocab][in]) bf16, None where not needed (a frozen head)."""
-    T, vocab = X.shape[0], W.shape[0]
-    with torch.cuda.device(X.device):
-        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_xent_workspace(T, X.shape[1], vocab))
-        _on(X.device, W, label, lse, g, ws)
-        lab, ls = _rows_of("label", label, (T,), torch.int32), _rows_of("lse", lse, (T,), torch.float32)
-        gp = _rows_of("g", g, (T,), torch.float32) if g is not None else None
-        dX = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device) if need_dx else None
-        dW = torch.empty(W.shape, dtype=torch.bfloat16, device=X.device) if need_dw else None
-        if T == 0:
-            return dX, dW.zero_() if need_dw else None
-        if need_dx or need_dw:
-            check(lib.k3gpu_lm_head_xent_grad(ptr(dX), X.shape[1], ptr(dW), gp, ls, X.data_ptr(), _row_stride(X), ptr(W),
-                                              lab, X.shape[1], vocab, T, ptr(ws), ws.numel(), stream_ptr(stream)),
-                  "k3gpu_lm_head_xent_grad")
+def _grads(X, W, need_dx, need_dw):
+    dX = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device) if need_dx else None
+    dW = torch.empty(W.shape, dtype=torch.bfloat16, device=X.device) if need_dw else None
+    if X.shape[0] == 0 and need_dw:
+        dW.zero_()
     return dX, dW
 
 
+@_on_device_of
+def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
+    """The gradient of lm_head_xent from its lse and the loss's incoming gradient g fp32 [T]
+    (None: 1): (dX [T][in], dW [vocab][in]) bf16, None where not needed (a frozen head)."""
+    xp, ldx, w, n, vocab, T = _head_args(X, W)
+    dev = X.device
+    lab, ls = _arg("label", label, dev, torch.int32, (T,)), _arg("lse", lse, dev, torch.float32, (T,))
+    gp = _arg("g", g, dev, torch.float32, (T,)) if g is not None else None
+    dX, dW = _grads(X, W, need_dx, need_dw)
+    if T and (need_dx or need_dw):
+        wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
+        check(lib.k3gpu_lm_head_xent_grad(ptr(dX), n, ptr(dW), gp, ls, xp, ldx, w, lab, n, vocab, T, wp, wn,
+                                          _stream_of(stream, dev)), "k3gpu_lm_head_xent_grad")
+    return dX, dW
+
+
+@_on_device_of
 def lm_head_distill(X, W, ids, top, temp=1.0, ws=None, stream=None):
     """KL of the teacher's top logits (ids int32, top fp32 [T][K], e.g. topk_logits of its
     sweep) from the head's softmax, both at temperature temp: (loss, lse) fp32 [T]. Entries with a
     negative id or a logit of -inf are empty; a row without entries has loss, lse and
     gradient 0."""
-    T, vocab, K = X.shape[0], W.shape[0], ids.shape[1]
-    with torch.cuda.device(X.device):
-        loss = torch.empty(T, dtype=torch.float32, device=X.device)
-        lse = torch.empty(T, dtype=torch.float32, device=X.device)
-        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_distill_workspace(T, X.shape[1], vocab, K))
-        _on(X.device, W, ids, top, ws)
-        ip, tp = _rows_of("ids", ids, (T, K), torch.int32), _rows_of("top", top, (T, K), torch.float32)
-        if T == 0:
-            return loss, lse
-        check(lib.k3gpu_lm_head_distill(ptr(loss), ptr(lse), X.data_ptr(), _row_stride(X), ptr(W), ip, tp, K, float(temp),
-                                        X.shape[1], vocab, T, ptr(ws), ws.numel(), stream_ptr(stream)),
-              "k3gpu_lm_head_distill")
+    xp, ldx, w, n, vocab, T = _head_args(X, W)
+    dev, K = X.device, ids.shape[-1]
+    ip, tp = _arg("ids", ids, dev, torch.int32, (T, K)), _arg("top", top, dev, torch.float32, (T, K))
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    lse = torch.empty(T, dtype=torch.float32, device=dev)
+    if T == 0:
+        return loss, lse
+    wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
+    check(lib.k3gpu_lm_head_distill(ptr(loss), ptr(lse), xp, ldx, w, ip, tp, K, float(temp), n, vocab, T, wp, wn,
+                                    _stream_of(stream, dev)), "k3gpu_lm_head_distill")
     return loss, lse
 
 
+@_on_device_of
 def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
     """The gradient of lm_head_distill (arguments and results as lm_head_xent_grad)."""
-    T, vocab, K = X.shape[0], W.shape[0], ids.shape[1]
-    with torch.cuda.device(X.device):
-        ws = _head_args(X, W, ws, lib.k3gpu_lm_head_distill_workspace(T, X.shape[1], vocab, K))
-        _on(X.device, W, ids, top, lse, g, ws)
-        ip, tp = _rows_of("ids", ids, (T, K), torch.int32), _rows_of("top", top, (T, K), torch.float32)
-        ls = _rows_of("lse", lse, (T,), torch.float32)
-        gp = _rows_of("g", g, (T,), torch.float32) if g is not None else None
-        dX = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device) if need_dx else None
-        dW = torch.empty(W.shape, dtype=torch.bfloat16, device=X.device) if need_dw else None
-        if T == 0:
-            return dX, dW.zero_() if need_dw else None
-        if need_dx or need_dw:
-            check(lib.k3gpu_lm_head_distill_grad(ptr(dX), X.shape[1], ptr(dW), gp, ls, X.data_ptr(), _row_stride(X),
-                                                 ptr(W), ip, tp, K, float(temp), X.shape[1], vocab, T, ptr(ws),
-                                                 ws.numel(), stream_ptr(stream)), "k3gpu_lm_head_distill_grad")
+    xp, ldx, w, n, vocab, T = _head_args(X, W)
+    dev, K = X.device, ids.shape[-1]
+    ip, tp = _arg("ids", ids, dev, torch.int32, (T, K)), _arg("top", top, dev, torch.float32, (T, K))
+    ls = _arg("lse", lse, dev, torch.float32, (T,))
+    gp = _arg("g", g, dev, torch.float32, (T,)) if g is not None else None
+    dX, dW = _grads(X, W, need_dx, need_dw)
+    if T and (need_dx or need_dw):
+        wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
+        check(lib.k3gpu_lm_head_distill_grad(ptr(dX), n, ptr(dW), gp, ls, xp, ldx, w, ip, tp, K, float(temp), n, vocab,
+                                             T, wp, wn, _stream_of(stream, dev)), "k3gpu_lm_head_distill_grad")
     return dX, dW
 
 

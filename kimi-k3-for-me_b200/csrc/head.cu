@@ -41,6 +41,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "pdl.cuh"
 #include "tc.cuh"
 
 namespace k3 {
@@ -438,6 +439,8 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
     sync_all<CG>();
     fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_release();
     const int n_live = *a.n_live;
     bool failed = false;
 
@@ -676,6 +679,8 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
     const int cols = (a.in + BN - 1) / BN, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row0 = (int)(blockIdx.x / cols) * BM, n0 = (int)(blockIdx.x % cols) * BN;
     const int row = row0 + ((w + 2) & 3) * 32 + lane, col = n0 + (w >> 2) * HALF + (int)blockIdx.y * 8;
+    pdl_wait();
+    pdl_release();
     if (row >= *a.n_live || col >= a.in) return;
     float4 f0 = make_float4(0, 0, 0, 0), f1 = f0;
     const float4 *p = a.acc + acc_at(a, 0, row0, n0, w) + (int)blockIdx.y * 64 + lane;
@@ -689,62 +694,91 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
     put8(a.dX + (size_t)a.row_of[row] * a.lddx + col, f0, f1, a.vec_dx);
 }
 
-// One block per row: the row's teacher entries as masses over ids in ascending order.
+// One warp per row: the row's teacher entries as masses over ids in ascending order.
 // An entry counts when its id lies in the vocabulary and its logit is not -inf;
 // mass = softmax(top / temp) over those. entropy = sum mass ln mass. The maximum carries a
 // NaN (fmaxf would drop it): such a row's masses, loss and gradient are NaN.
-__global__ void __launch_bounds__(MAXK) teacher_kernel(int *__restrict__ s_ids, float *__restrict__ s_mass,
-                                                       int *__restrict__ count, float *__restrict__ entropy,
-                                                       const int *__restrict__ ids, const float *__restrict__ top,
-                                                       int K, int vocab, float inv_temp)
+constexpr int TEACHER_ROWS = 4, PER_LANE = MAXK / 32;
+__global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *__restrict__ s_ids, float *__restrict__ s_mass,
+                                                                    int *__restrict__ count,
+                                                                    float *__restrict__ entropy,
+                                                                    const int *__restrict__ ids,
+                                                                    const float *__restrict__ top, int T, int K,
+                                                                    int vocab, float inv_temp)
 {
-    __shared__ int sid[MAXK];
-    __shared__ float st[MAXK];
-    __shared__ double se[MAXK];
-    const size_t base = (size_t)blockIdx.x * K;
-    const int k = threadIdx.x;
-    int id = -1;
-    float t = -INFINITY;
-    if (k < K) {
-        id = ids[base + k];
-        t = top[base + k];
-        if (id >= vocab) flag(DEV_BAD_INDEX);
-    }
-    const bool ok = id >= 0 && id < vocab && t != -INFINITY;
-    sid[k] = ok ? id : -1;
-    st[k] = ok ? t : -INFINITY;
-    __syncthreads();
+    __shared__ __align__(16) int sid_all[TEACHER_ROWS][MAXK];
+    pdl_wait();
+    pdl_release();
+    const int lane = threadIdx.x & 31, row = blockIdx.x * TEACHER_ROWS + (threadIdx.x >> 5);
+    if (row >= T) return;
+    int *sid = sid_all[threadIdx.x >> 5];
+    const size_t base = (size_t)row * K;
+    int id[PER_LANE], place[PER_LANE];
+    float t[PER_LANE], e[PER_LANE];
     float mx = -INFINITY;
-    int nan = 0;
-    for (int j = 0; j < K; j++) {
-        nan |= st[j] != st[j];
-        mx = fmaxf(mx, st[j]);
+    bool nan = false;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; i++) {
+        const int k = lane + 32 * i;
+        id[i] = k < K ? ids[base + k] : -1;
+        t[i] = k < K ? top[base + k] : -INFINITY;
+        if (id[i] >= vocab) {
+            flag(DEV_BAD_INDEX);
+            id[i] = -1;
+        }
+        if (id[i] < 0 || t[i] == -INFINITY) id[i] = 0x7fffffff;    // empty: behind every id
+        else {
+            n++;
+            nan |= t[i] != t[i];
+            mx = fmaxf(mx, t[i]);
+        }
+        sid[k] = id[i];
+        place[i] = 0;
     }
-    if (nan) mx = NAN;
-    const double l = ok ? ((double)st[k] - (double)mx) * (double)inv_temp : 0.0;
-    const double e = ok ? exp(l) : 0.0;
-    se[k] = e;
-    __syncthreads();
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (__any_sync(0xffffffffu, nan)) mx = NAN;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, mx, o);
+        mx = mx != mx ? mx : fmaxf(mx, other);
+    }
     double sum = 0.0;
-    int place = 0, n = 0;
-    for (int j = 0; j < K; j++) {
-        sum += se[j];
-        n += sid[j] >= 0;
-        place += sid[j] >= 0 && (sid[j] < id || (sid[j] == id && j < k));
+#pragma unroll
+    for (int i = 0; i < PER_LANE; i++) {
+        t[i] = (t[i] - mx) * inv_temp;
+        e[i] = id[i] != 0x7fffffff ? expf(t[i]) : 0.0f;
+        sum += (double)e[i];
     }
-    const double m = e / sum;
-    if (ok) {
-        s_ids[base + place] = id;
-        s_mass[base + place] = (float)m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncwarp();
+    // each entry's place among the ids; equal ids by position
+    const int used = (K + 31) & ~31;
+    for (int j = 0; j < used; j += 4) {
+        const int4 o = *reinterpret_cast<const int4 *>(sid + j);
+#pragma unroll
+        for (int i = 0; i < PER_LANE; i++) {
+            const int k = lane + 32 * i;
+            place[i] += (o.x < id[i] || (o.x == id[i] && j < k)) + (o.y < id[i] || (o.y == id[i] && j + 1 < k)) +
+                        (o.z < id[i] || (o.z == id[i] && j + 2 < k)) + (o.w < id[i] || (o.w == id[i] && j + 3 < k));
+        }
     }
-    __syncthreads();
-    se[k] = ok ? (e == 0.0 ? 0.0 : m * (l - log(sum))) : 0.0;
-    __syncthreads();
-    if (k == 0) {
-        double h = 0.0;
-        for (int j = 0; j < K; j++) h += se[j];
-        count[blockIdx.x] = n;
-        entropy[blockIdx.x] = (float)h;
+    const double log_sum = log(sum);
+    double h = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; i++)
+        if (id[i] != 0x7fffffff) {
+            const double m = (double)e[i] / sum;
+            s_ids[base + place[i]] = id[i];
+            s_mass[base + place[i]] = (float)m;
+            if (e[i] != 0.0f) h += m * ((double)t[i] - log_sum);   // (a NaN is not equal to 0)
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) h += __shfl_xor_sync(0xffffffffu, h, o);
+    if (lane == 0) {
+        count[row] = n;
+        entropy[row] = (float)h;
     }
 }
 
@@ -763,6 +797,8 @@ __global__ void __launch_bounds__(256) pack_kernel(int *__restrict__ row_of, int
     __shared__ int red[2][8];
     __shared__ int place[PACK_ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    pdl_release();
     const int t0 = blockIdx.x * rows, t1 = min(T, t0 + rows);
     auto counts = [&](int t) {
         if (!label) return count[t] > 0;
@@ -837,14 +873,24 @@ __global__ void __launch_bounds__(1024) join_kernel(float *__restrict__ loss, fl
     __shared__ float sm[32][33];
     __shared__ float ss[32][33];
     const int r = threadIdx.x & 31, w = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_release();
     const int row = blockIdx.x * 32 + r, n = *n_live;
     if ((int)blockIdx.x * 32 >= n) return;
     float m = -INFINITY, s = 0.0f;
     if (row < n)
-        for (int h = w; h < halves; h += 32) {
-            const float2 p = part[(size_t)h * Tpad + row];
-            const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.0f : mn;
-            s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
+        for (int h = w; h < halves; h += 32 * 8) {
+            float2 p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                p[i] = h + 32 * i < halves ? part[(size_t)(h + 32 * i) * Tpad + row] : make_float2(-INFINITY, 0.0f);
+            float mn = m;
+#pragma unroll
+            for (int i = 0; i < 8; i++) mn = fmaxf(mn, p[i].x);
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            s *= exp2f(m - ref);
+#pragma unroll
+            for (int i = 0; i < 8; i++) s += p[i].y * exp2f(p[i].x - ref);
             m = mn;
         }
     sm[w][r] = m;
@@ -1053,21 +1099,20 @@ struct Call {
 
 // The targets, the rows that count and their hidden states; fills the common arguments.
 static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w, float *loss, float *lse,
-                  uint16_t *dX, int lddx, int cg)
+                  uint16_t *dX, int lddx, int cg, bool grad)
 {
     int st;
     if (c.K) {
-        teacher_kernel<<<c.T, MAXK, 0, c.s>>>(w.ids, w.mass, w.count, w.entropy, c.ids, c.top, c.K, c.vocab,
-                                              1.0f / c.temp);
-        if ((st = launch_status())) return st;
+        st = launch_pdl(teacher_kernel, dim3(ceil_div(c.T, TEACHER_ROWS)), 32 * TEACHER_ROWS, 0, c.s, 1, w.ids, w.mass,
+                        w.count, w.entropy, c.ids, c.top, c.T, c.K, c.vocab, 1.0f / c.temp);
+        if (st) return st;
     }
     const int in_place = c.ldx % 8 == 0 && aligned(c.X, 16);
     const int rows = std::max(8, ceil_div(c.T, PACK_BLOCKS));
-    pack_kernel<<<ceil_div(c.T, rows), 256, 0, c.s>>>(w.row_of, w.n_live, w.xp, loss, lse,
-                                                      reinterpret_cast<__nv_bfloat16 *>(dX), lddx, c.X, c.ldx,
-                                                      in_place, c.K ? nullptr : c.label, w.count, c.T, c.in, c.vocab,
-                                                      rows);
-    if ((st = launch_status())) return st;
+    st = launch_pdl(pack_kernel, dim3(ceil_div(c.T, rows)), 256, 0, c.s, 1, w.row_of, w.n_live, w.xp, loss, lse,
+                    reinterpret_cast<__nv_bfloat16 *>(dX), lddx, c.X, c.ldx, in_place, c.K ? nullptr : c.label, w.count,
+                    c.T, c.in, c.vocab, rows);
+    if (st) return st;
     *a = Args{};
     a->T = c.T; a->in = c.in;
     a->n_live = w.n_live; a->row_of = w.row_of; a->Tpad = p.Tpad;
@@ -1082,34 +1127,18 @@ static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w
     const void *x = in_place ? (const void *)c.X : (const void *)w.xp;
     const long long ldx = in_place ? c.ldx : c.in, xr = in_place ? c.T : p.Tpad;
     if ((st = map2d(&maps->x_k, x, c.in, ldx, xr, BM))) return st;
-    if ((st = map2d(&maps->x_mn, x, c.in, ldx, xr, 64))) return st;
     if ((st = map2d(&maps->xp_k, w.xp, c.in, c.in, p.Tpad, BM))) return st;
-    if ((st = map2d(&maps->xp_mn, w.xp, c.in, c.in, p.Tpad, 64))) return st;
     if ((st = map2d(&maps->w_k, c.W, c.in, c.in, c.vocab, BN / cg))) return st;
+    if (!grad) return K3GPU_OK;
+    if ((st = map2d(&maps->x_mn, x, c.in, ldx, xr, 64))) return st;
+    if ((st = map2d(&maps->xp_mn, w.xp, c.in, c.in, p.Tpad, 64))) return st;
     return map2d(&maps->w_mn, c.W, c.in, c.in, c.vocab, 64);
 }
 
 template <int MODE, int CG>
 static int launch_head(const Maps &maps, const Args &a, int sms, cudaStream_t s)
 {
-    if (CG == 1) {
-        head_kernel<MODE, CG><<<sms, THREADS, SMEM, s>>>(maps, a);
-        return launch_status();
-    }
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = CG;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(sms / CG * CG);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SMEM;
-    cfg.stream = s;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, head_kernel<MODE, CG>, maps, a);
-    const int st = launch_status();
-    return e != cudaSuccess ? cuda_status(e) : st;
+    return launch_pdl(head_kernel<MODE, CG>, dim3(sms / CG * CG), THREADS, SMEM, s, CG, maps, a);
 }
 
 static int forward(float *loss, float *lse, const Call &c, void *ws)
@@ -1121,13 +1150,12 @@ static int forward(float *loss, float *lse, const Call &c, void *ws)
     layout(&w, static_cast<char *>(ws), p, c.T, c.in, c.K, false);
     Args a;
     Maps maps{};
-    if ((st = set_up(&a, &maps, c, p, w, loss, lse, nullptr, 0, 1))) return st;
+    if ((st = set_up(&a, &maps, c, p, w, loss, lse, nullptr, 0, 1, false))) return st;
     a.part = w.part; a.zt = w.zt;
     a.z = Piece{0, c.vocab, nullptr};
     if ((st = launch_head<LOSS, 1>(maps, a, sms, c.s))) return st;
-    join_kernel<<<p.Tpad / 32, 1024, 0, c.s>>>(loss, lse, w.part, 2 * p.tiles, p.Tpad, w.row_of, w.n_live, w.zt, w.mass,
-                                               w.count, w.entropy, a.K, a.inv_temp);
-    return launch_status();
+    return launch_pdl(join_kernel, dim3(p.Tpad / 32), 1024, 0, c.s, 1, loss, lse, w.part, 2 * p.tiles, p.Tpad, w.row_of,
+                      w.n_live, w.zt, w.mass, w.count, w.entropy, a.K, a.inv_temp);
 }
 
 // Launch i forms piece i's dz beside the dX and dW of piece i - 1 (two dz buffers), so each
@@ -1141,7 +1169,7 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     layout(&w, static_cast<char *>(ws), p, c.T, c.in, c.K, true);
     Args a;
     Maps maps{};
-    if ((st = set_up(&a, &maps, c, p, w, nullptr, nullptr, dX, lddx, p.cg))) return st;
+    if ((st = set_up(&a, &maps, c, p, w, nullptr, nullptr, dX, lddx, p.cg, true))) return st;
     a.lse = lse; a.g = g;
     a.acc = w.acc;
     a.splits = p.splits; a.split_steps = p.split_steps;
@@ -1164,8 +1192,7 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
         if (st) return st;
     }
     if (dX && p.splits > 1) {
-        sum_splits_kernel<<<dim3(ceil_div(c.T, BM) * ceil_div(c.in, BN), HALF / 8), 256, 0, c.s>>>(a);
-        return launch_status();
+        return launch_pdl(sum_splits_kernel, dim3(ceil_div(c.T, BM) * ceil_div(c.in, BN), HALF / 8), 256, 0, c.s, 1, a);
     }
     return K3GPU_OK;
 }

@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "pdl.cuh"
 
 namespace k3 {
 namespace topk {
@@ -187,6 +188,8 @@ __global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restric
     const int begin = blockIdx.x * seg_len, end = min(vocab, begin + seg_len);
     if (threadIdx.x == 0) { s.n = s.n_quads = 0; s.bar = 0; }
     __syncthreads();
+    pdl_wait();
+    pdl_release();
     // quads lie on 16-byte boundaries; the first may start before the segment
     const int skew = (int)((reinterpret_cast<uintptr_t>(row + begin) & 15u) / 4);
     int n = 0;
@@ -274,6 +277,8 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(int *__restrict__ idx, f
     const int total = nseg * K;
     cand += (size_t)blockIdx.x * total;
     if (threadIdx.x == 0) s.n = 0;
+    pdl_wait();
+    pdl_release();
     uint64_t r[MERGE];
     uint32_t most = 0;
 #pragma unroll
@@ -329,9 +334,8 @@ extern "C" int k3gpu_topk_logits(int *idx, float *val, const float *logits, int 
     const int seg_len = k3::ceil_div(k3::ceil_div(vocab, nseg), 4) * 4;
     uint64_t *cand = static_cast<uint64_t *>(workspace);
     cudaStream_t s = k3::as_stream(stream);
-    segment_kernel<<<dim3(nseg, rows), THREADS, 0, s>>>(cand, idx, val, logits, vocab, seg_len, K);
-    const int st = k3::launch_status();
+    const int st = k3::launch_pdl(segment_kernel, dim3(nseg, rows), THREADS, 0, s, 1, cand, idx, val, logits, vocab,
+                                  seg_len, K);
     if (st || nseg == 1) return st;
-    merge_kernel<<<rows, THREADS, 0, s>>>(idx, val, cand, nseg, K);
-    return k3::launch_status();
+    return k3::launch_pdl(merge_kernel, dim3(rows), THREADS, 0, s, 1, idx, val, cand, nseg, K);
 }
