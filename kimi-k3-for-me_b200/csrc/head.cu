@@ -79,13 +79,12 @@ struct Piece {
 struct Args {
     int T, in;
     const int *n_live;          // rows that count
-    const int *row_of;          // [T] packed row -> row
+    const int4 *rows;           // [T] of a packed row: its row t, its label or count of entries, lse log2(e), weight
     int Tpad;
     int x_in_place;             // X itself can be read by TMA when every row counts
     // targets, by row: entry e of row t is ids[t * K + e] (ascending), mass[t * K + e]
-    const int *ids;
-    const float *mass;          // nullptr: cross entropy (K = 1, mass 1)
-    const int *count;           // entries of a row; nullptr: 1
+    const int *ids;             // nullptr: cross entropy (K = 1, mass 1, the label in `rows`)
+    const float *mass;
     int K;
     float c;                    // log2(e) / temp
     Piece z;                    // vc = 0: no z units in this launch
@@ -93,7 +92,7 @@ struct Args {
     float2 *part;               // [2 * vocabulary tiles][Tpad] (max, sum), base 2
     float *zt;                  // [T][K] z of the targets
     // GRAD
-    const float *lse, *g;       // by row; g may be nullptr (1)
+    const float *g_scale;       // what the weights in `rows` were divided by; nullptr: nothing
     float inv_temp;
     Piece d;                    // vc = 0: no dX and dW units in this launch
     int want_dx, want_dw, first, last;
@@ -304,22 +303,26 @@ __device__ __forceinline__ int first_entry(const int *ids, int cnt, int v)
     return lo;
 }
 
-// One unit's z in registers: the thread's row, HALF columns from col0 of the piece. What the row
-// needs was fetched before the products were done.
+// The targets of the thread's row from the unit's column col0 on.
 struct RowTargets {
-    const int *ids;
     int e, cnt, next;           // the next entry, entries, the next entry's column in the piece
-    __device__ __forceinline__ void start(const Args &a, int t, bool live, int col0)
+    __device__ __forceinline__ void start(const Args &a, const int4 &r, bool live, int col0)
     {
-        ids = a.ids + (size_t)t * a.K;
-        cnt = live ? (a.count ? a.count[t] : 1) : 0;
+        if (!a.ids) {
+            e = 0;
+            cnt = 1;
+            next = live && r.y - a.z.v0 >= col0 ? r.y - a.z.v0 : 0x7fffffff;
+            return;
+        }
+        const int *ids = a.ids + (size_t)r.x * a.K;
+        cnt = live ? r.y : 0;
         e = first_entry(ids, cnt, a.z.v0 + col0);
         next = e < cnt ? ids[e] - a.z.v0 : 0x7fffffff;
     }
-    __device__ __forceinline__ void step(const Args &a)
+    __device__ __forceinline__ void step(const Args &a, int t)
     {
         e++;
-        next = e < cnt ? ids[e] - a.z.v0 : 0x7fffffff;
+        next = e < cnt ? a.ids[(size_t)t * a.K + e] - a.z.v0 : 0x7fffffff;
     }
 };
 
@@ -335,19 +338,20 @@ __device__ __forceinline__ void loss_epilogue(const Args &a, float (&z)[HALF], R
             for (int j = 0; j < 32; j++)
                 if (at & (1u << j)) v = z[c0 + j];
             a.zt[(size_t)t * a.K + tg.e] = v;
-            tg.step(a);
+            tg.step(a, t);
         }
     const int left = a.z.vc - col0;
+    if (left < HALF) {                     // the vocabulary ends here
+#pragma unroll
+        for (int j = 0; j < HALF; j++) z[j] = j < left ? z[j] : -INFINITY;
+    }
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int j = 0; j < HALF; j++) {
-        z[j] = j < left ? z[j] * a.c : -INFINITY;
-        mx[j & 3] = fmaxf(mx[j & 3], z[j]);
-    }
-    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), ref = m == -INFINITY ? 0.0f : m;
+    for (int j = 0; j < HALF; j += 2) mx[(j >> 1) & 3] = fmaxf(mx[(j >> 1) & 3], fmaxf(z[j], z[j + 1]));
+    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.c, ref = m == -INFINITY ? 0.0f : m;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < HALF; j++) s[j & 3] += ex2(z[j] - ref);
+    for (int j = 0; j < HALF; j++) s[j & 3] += ex2(fmaf(z[j], a.c, -ref));
     if (live) a.part[(size_t)(col0 / HALF) * a.Tpad + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
@@ -365,29 +369,35 @@ __device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *ou
 #pragma unroll
             for (int j = 0; j < 32; j++)
                 if (at & (1u << j)) z[c0 + j] -= q;
-            tg.step(a);
+            tg.step(a, t);
         }
     // rows of the tile past the live ones are zeros: dW sums over them
-    const float gz = live ? gt : 0.0f;
+    if (!live) {
+#pragma unroll
+        for (int j = 0; j < HALF; j++) z[j] = 0.0f;
+        gt = 0.0f;
+    }
 #pragma unroll
     for (int c0 = 0; c0 < HALF; c0 += 64)
         store64(buf, out, col0 + c0, row0, false, lane, [&](int j) {
             const float *f = z + c0 + 8 * j;
-            if (!live) return make_uint4(0u, 0u, 0u, 0u);
-            return make_uint4(pack_bf16(f[0] * gz, f[1] * gz), pack_bf16(f[2] * gz, f[3] * gz),
-                              pack_bf16(f[4] * gz, f[5] * gz), pack_bf16(f[6] * gz, f[7] * gz));
+            return make_uint4(pack_bf16(f[0] * gt, f[1] * gt), pack_bf16(f[2] * gt, f[3] * gt),
+                              pack_bf16(f[4] * gt, f[5] * gt), pack_bf16(f[6] * gt, f[7] * gt));
         });
 }
 
+// dz was formed without these: exactly common factors add no rounding of their own to it
+__device__ __forceinline__ float out_scale(const Args &a) { return (a.g_scale ? *a.g_scale : 1.0f) * a.inv_temp; }
 // where a warp's part of a dX tile lies in acc (float4s; its lanes follow)
 __device__ __forceinline__ size_t acc_at(const Args &a, int split, int row0, int col0, int w)
 {
     const size_t tile = ((size_t)split * (a.Tpad / BM) + row0 / BM) * ((a.in + BN - 1) / BN) + col0 / BN;
     return (tile * 8 + w) * (HALF / 4) * 32;
 }
-__device__ __forceinline__ void put8(__nv_bfloat16 *out, const float4 &f0, const float4 &f1, bool vec)
+__device__ __forceinline__ void put8(__nv_bfloat16 *out, const float4 &f0, const float4 &f1, float k, bool vec)
 {
-    const uint4 o = make_uint4(pack_bf16(f0.x, f0.y), pack_bf16(f0.z, f0.w), pack_bf16(f1.x, f1.y), pack_bf16(f1.z, f1.w));
+    const uint4 o = make_uint4(pack_bf16(f0.x * k, f0.y * k), pack_bf16(f0.z * k, f0.w * k),
+                               pack_bf16(f1.x * k, f1.y * k), pack_bf16(f1.z * k, f1.w * k));
     if (vec) {
         *reinterpret_cast<uint4 *>(out) = o;
     } else {
@@ -551,51 +561,59 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
             }
             use++;
         };
-        for (int n_units = 0; !failed; n_units++) {
+        // the next unit, and of its packed row what `rows` says (on its way while this one ends)
+        int n_units = 0;
+        auto take = [&](int4 &words, int4 &r) {
             const int slot = n_units % NU;
-            if (!bar_wait(s_addr(&b_unit[slot]), (uint32_t)((n_units / NU) & 1))) { failed = true; break; }
-            const Unit t = Unit::of(unit_slot[slot]);
+            words.x = -1;
+            if (!bar_wait(s_addr(&b_unit[slot]), (uint32_t)((n_units / NU) & 1))) { failed = true; return; }
+            n_units++;
+            words = unit_slot[slot];
             __syncwarp();
             if (lane == 0) bar_arrive(s_addr(&b_took[slot]));
-            if (t.kind < 0) break;
+            const int row = words.y + rank * BM + q * 32 + lane;
+            if (words.x >= 0 && row < n_live) r = __ldg(a.rows + row);   // (of a dW unit it means nothing)
+        };
+        int4 words, words_next, r = make_int4(0, 0, 0, 0), r_next = r;
+        for (take(words, r); words.x >= 0 && !failed; words = words_next, r = r_next) {
+            const Unit t = Unit::of(words);
             const int row0 = t.m0 + rank * BM + q * 32, row = row0 + lane;   // packed row (z, dX), id of the piece (dW)
             const int col0 = t.n0 + half * HALF;
             const uint32_t src = tmem + lanes + (uint32_t)(half * HALF);
             if (MODE == LOSS || t.kind == Z) {
-                // what the row needs is fetched while the unit's products run
                 const bool live = row < n_live;
-                const int tr = live ? a.row_of[row] : 0;
                 RowTargets tg;
-                tg.start(a, tr, live, col0);
-                float l2 = 0.0f, gt = 0.0f;
-                if (MODE == GRAD && live) {
-                    l2 = a.lse[tr] * LOG2E;
-                    gt = (a.g ? a.g[tr] : 1.0f) * a.inv_temp;
-                }
+                tg.start(a, r, live, col0);
                 float z[HALF];
-#pragma unroll
-                for (int j = 0; j < HALF; j++) z[j] = 0.0f;
                 __syncwarp();
+                if (!finished()) { failed = true; break; }
+#pragma unroll
+                for (int c0 = 0; c0 < HALF; c0 += 32)
+                    tmem_ld32(src + (uint32_t)((use & 1) * BN + c0), *reinterpret_cast<uint32_t(*)[32]>(z + c0));
+                tmem_wait_ld();
+                release();
 #pragma unroll 1
-                for (int ks = 0; ks < t.steps; ks += Z_CHUNK) {
+                for (int ks = Z_CHUNK; ks < t.steps; ks += Z_CHUNK) {
                     if (!finished()) { failed = true; break; }
-                    const uint32_t at = src + (uint32_t)((use & 1) * BN);
 #pragma unroll
                     for (int c0 = 0; c0 < HALF; c0 += 16) {
                         uint32_t v[16];
-                        tmem_ld16(at + (uint32_t)c0, v);
+                        tmem_ld16(src + (uint32_t)((use & 1) * BN + c0), v);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            z[c0 + j] += __uint_as_float(v[j]);
+                        for (int j = 0; j < 16; j++) z[c0 + j] += __uint_as_float(v[j]);
                     }
                     release();
                 }
                 if (failed) break;
-                if (MODE == LOSS) loss_epilogue(a, z, tg, tr, row, live, col0);
-                else dz_epilogue(a, &maps.z_out, buf, z, tg, tr, row0, lane, live, col0, l2, gt);
+                if (MODE == LOSS) take(words_next, r_next);
+                if (MODE == LOSS) loss_epilogue(a, z, tg, r.x, row, live, col0);
+                else dz_epilogue(a, &maps.z_out, buf, z, tg, r.x, row0, lane, live, col0, __int_as_float(r.z), __int_as_float(r.w));
                 __syncwarp();
+                if (MODE != LOSS) take(words_next, r_next);
             } else if (t.kind == DW) {
+                const float scale = out_scale(a);
+                take(words_next, r_next);
                 if (t.steps > 0 && !finished()) { failed = true; break; }
                 for (int c0 = 0; c0 < HALF; c0 += 64) {
                     uint32_t v[2][32];
@@ -611,15 +629,17 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                     const int col = col0 + c0;
                     store64(buf, &maps.w_out, col, a.d.v0 + row0, col >= a.in || row0 >= a.d.vc, lane, [&](int j) {
                         const uint32_t *f = v[j >> 2] + 8 * (j & 3);
-                        auto pk = [&](int k) { return pack_bf16(__uint_as_float(f[k]), __uint_as_float(f[k + 1])); };
+                        auto pk = [&](int k) { return pack_bf16(__uint_as_float(f[k]) * scale, __uint_as_float(f[k + 1]) * scale); };
                         return make_uint4(pk(0), pk(2), pk(4), pk(6));
                     });
                 }
             } else {
                 const bool live = row < n_live;
+                const float scale = out_scale(a);
                 const bool sum = a.splits > 1 || !a.last, add = !a.first;
                 float4 *acc = a.acc + acc_at(a, t.split, t.m0 + rank * BM, t.n0, warp - 2) + lane;
-                __nv_bfloat16 *out = live ? a.dX + (size_t)a.row_of[row] * a.lddx : nullptr;
+                __nv_bfloat16 *out = live ? a.dX + (size_t)r.x * a.lddx : nullptr;
+                take(words_next, r_next);
                 if (t.steps > 0 && !finished()) { failed = true; break; }
                 for (int c0 = 0; c0 < HALF; c0 += 32) {
                     uint32_t v[32];
@@ -649,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                             acc[at] = f0;
                             acc[at + 32] = f1;
                         } else if (col0 + c0 + j < a.in) {
-                            put8(out + col0 + c0 + j, f0, f1, a.vec_dx);
+                            put8(out + col0 + c0 + j, f0, f1, scale, a.vec_dx);
                         }
                     }
                 }
@@ -691,7 +711,7 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
         f0.x += p0.x; f0.y += p0.y; f0.z += p0.z; f0.w += p0.w;
         f1.x += p1.x; f1.y += p1.y; f1.z += p1.z; f1.w += p1.w;
     }
-    put8(a.dX + (size_t)a.row_of[row] * a.lddx + col, f0, f1, a.vec_dx);
+    put8(a.dX + (size_t)a.rows[row].x * a.lddx + col, f0, f1, out_scale(a), a.vec_dx);
 }
 
 // One warp per row: the row's teacher entries as masses over ids in ascending order.
@@ -782,92 +802,117 @@ __global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *__restr
     }
 }
 
-// Numbers the rows that count, in order (row_of[place] = t, *n_live), copies their hidden
-// states to their places and writes zeros for the others' outputs. Each block takes `rows`
-// rows and counts the live ones before them itself (T * 4 bytes from L2, at most PACK_BLOCKS
-// blocks), so one launch does it. When every row counts and X can be read in place nothing
-// is copied; else the rows from the last packed one to the end of its tile become zeros.
-__global__ void __launch_bounds__(256) pack_kernel(int *__restrict__ row_of, int *__restrict__ n_live,
-                                                   __nv_bfloat16 *__restrict__ Xp, float *__restrict__ loss,
-                                                   float *__restrict__ lse, __nv_bfloat16 *__restrict__ dX, int lddx,
-                                                   const uint16_t *__restrict__ X, int ldx, int in_place,
-                                                   const int *__restrict__ label, const int *__restrict__ count,
-                                                   int T, int in, int vocab, int rows)
+// Numbers the rows that count, in order (rows[place], *n_live), copies their hidden states to
+// their places and writes zeros for the others' outputs. Each block takes `per` rows and
+// counts the live ones before them itself (T * 4 bytes from L2, at most PACK_BLOCKS blocks),
+// so one launch does it. When every row counts and X can be read in place nothing is copied;
+// else the rows from the last packed one to the end of its tile become zeros.
+// The weights are divided by the largest of them (*g_scale): a mean's common 1 / n then
+// rounds nothing when dz becomes bf16. (Where the largest is 0 or not finite, by 1.)
+struct Pack {
+    int4 *rows;
+    int *n_live;
+    float *g_scale;
+    uint16_t *xp;
+    float *loss, *lse_out;             // forward
+    __nv_bfloat16 *dX;                 // backward
+    const float *lse, *g;
+    const uint16_t *X;
+    const int *label, *count;          // one of them
+    int lddx, ldx, in_place, T, in, vocab, per;
+};
+
+__global__ void __launch_bounds__(256) pack_kernel(const Pack k)
 {
     __shared__ int red[2][8];
+    __shared__ float red_g[8];
     __shared__ int place[PACK_ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_release();
-    const int t0 = blockIdx.x * rows, t1 = min(T, t0 + rows);
+    const int T = k.T, in = k.in, t0 = blockIdx.x * k.per, t1 = min(T, t0 + k.per);
     auto counts = [&](int t) {
-        if (!label) return count[t] > 0;
-        const int l = label[t];
-        return l >= 0 && l < vocab;
+        if (!k.label) return k.count[t] > 0;
+        const int l = k.label[t];
+        return l >= 0 && l < k.vocab;
     };
     int before = 0, total = 0;
+    float g_max = 0.0f;
     for (int t = tid; t < T; t += 256) {
         const int c = counts(t);
         total += c;
         before += t < t0 ? c : 0;
+        if (c && k.g) g_max = fmaxf(g_max, fabsf(k.g[t]));
     }
     before = __reduce_add_sync(0xffffffffu, before);
     total = __reduce_add_sync(0xffffffffu, total);
-    if (lane == 0) { red[0][warp] = before; red[1][warp] = total; }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) g_max = fmaxf(g_max, __shfl_xor_sync(0xffffffffu, g_max, o));
+    if (lane == 0) { red[0][warp] = before; red[1][warp] = total; red_g[warp] = g_max; }
     __syncthreads();
     before = total = 0;
 #pragma unroll
-    for (int w = 0; w < 8; w++) { before += red[0][w]; total += red[1][w]; }
+    for (int w = 0; w < 8; w++) {
+        before += red[0][w];
+        total += red[1][w];
+        g_max = fmaxf(g_max, red_g[w]);
+    }
+    const float g_scale = k.g && g_max > 0.0f && g_max < INFINITY ? g_max : 1.0f;
     if (warp == 0) {
         for (int b = t0; b < t1; b += 32) {
             const int t = b + lane;
             const bool live = t < t1 && counts(t);
-            if (t < t1 && label && label[t] >= vocab) flag(DEV_BAD_INDEX);
+            if (t < t1 && k.label && k.label[t] >= k.vocab) flag(DEV_BAD_INDEX);
             const unsigned m = __ballot_sync(0xffffffffu, live);
             const int p = before + __popc(m & ((1u << lane) - 1));
             if (t < t1) place[t - t0] = live ? p : -1;
-            if (live) row_of[p] = t;
+            if (live) {
+                const float l2 = k.lse ? k.lse[t] * LOG2E : 0.0f, g = k.g ? k.g[t] / g_scale : 1.0f;
+                k.rows[p] = make_int4(t, k.label ? k.label[t] : k.count[t], __float_as_int(l2), __float_as_int(g));
+            }
             before += __popc(m);
         }
     }
-    if (blockIdx.x == 0 && tid == 0) *n_live = total;
+    if (blockIdx.x == 0 && tid == 0) {
+        *k.n_live = total;
+        *k.g_scale = g_scale;
+    }
     __syncthreads();
-    const bool copy = !(in_place && total == T);
-    uint16_t *xp = reinterpret_cast<uint16_t *>(Xp);
+    const bool copy = !(k.in_place && total == T);
     for (int t = t0 + warp; t < t1; t += 8) {
         const int p = place[t - t0];
         if (p >= 0) {
             if (!copy) continue;
-            const uint16_t *x = X + (size_t)t * ldx;
-            if (in_place) {                        // rows 16-byte aligned
+            const uint16_t *x = k.X + (size_t)t * k.ldx;
+            if (k.in_place) {                      // rows 16-byte aligned
 #pragma unroll 4
                 for (int i = lane; i < in / 8; i += 32)
-                    reinterpret_cast<uint4 *>(xp + (size_t)p * in)[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
+                    reinterpret_cast<uint4 *>(k.xp + (size_t)p * in)[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
             } else {
 #pragma unroll 4
-                for (int i = lane; i < in; i += 32) xp[(size_t)p * in + i] = __ldg(x + i);
+                for (int i = lane; i < in; i += 32) k.xp[(size_t)p * in + i] = __ldg(x + i);
             }
             continue;
         }
-        if (loss && lane == 0) {
-            loss[t] = 0.0f;
-            lse[t] = 0.0f;
+        if (k.loss && lane == 0) {
+            k.loss[t] = 0.0f;
+            k.lse_out[t] = 0.0f;
         }
-        if (dX)
-            for (int i = lane; i < in; i += 32) dX[(size_t)t * lddx + i] = __float2bfloat16_rn(0.0f);
+        if (k.dX)
+            for (int i = lane; i < in; i += 32) k.dX[(size_t)t * k.lddx + i] = __float2bfloat16_rn(0.0f);
     }
     if (copy)
-        for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + ROW_PAD - 1) / ROW_PAD * ROW_PAD; p += (int)gridDim.x * 8)
+        for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
+             p += (int)gridDim.x * 8)
             for (int i = lane; i < in / 8; i += 32)
-                reinterpret_cast<uint4 *>(xp + (size_t)p * in)[i] = make_uint4(0u, 0u, 0u, 0u);
+                reinterpret_cast<uint4 *>(k.xp + (size_t)p * in)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // 32 packed rows a block, 32 threads a row: the tile halves' statistics joined in double.
 __global__ void __launch_bounds__(1024) join_kernel(float *__restrict__ loss, float *__restrict__ lse,
                                                     const float2 *__restrict__ part, int halves, int Tpad,
-                                                    const int *__restrict__ row_of, const int *__restrict__ n_live,
+                                                    const int4 *__restrict__ rows, const int *__restrict__ n_live,
                                                     const float *__restrict__ zt, const float *__restrict__ mass,
-                                                    const int *__restrict__ count,
                                                     const float *__restrict__ entropy, int K, float inv_temp)
 {
     __shared__ float sm[32][33];
@@ -905,8 +950,8 @@ __global__ void __launch_bounds__(1024) join_kernel(float *__restrict__ loss, fl
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ref = M == -INFINITY ? 0.0f : M;
     double S = (double)ls * exp2((double)lm - (double)ref);
-    const int t = row_of[mine];
-    const int cnt = count ? count[t] : 1;
+    const int4 info = rows[mine];
+    const int t = info.x, cnt = mass ? info.y : 1;
     double zq = 0.0;
     for (int e = r; e < cnt; e += 32) {
         const double q = mass ? (double)mass[(size_t)t * K + e] : 1.0;
@@ -1027,8 +1072,9 @@ static Plan plan(int T, int in, int vocab)
 }
 
 struct Ws {
-    int *n_live, *row_of, *ids, *count;
-    float *mass, *entropy, *zt;
+    int *n_live, *ids, *count;
+    int4 *rows;
+    float *g_scale, *mass, *entropy, *zt;
     float4 *acc;
     float2 *part;
     __nv_bfloat16 *xp, *dz[2];
@@ -1045,7 +1091,8 @@ static size_t layout(Ws *w, char *base, const Plan &p, int T, int in, int K, boo
     };
     Ws x{};
     x.n_live = (int *)take(4);
-    x.row_of = (int *)take((size_t)T * 4);
+    x.g_scale = (float *)take(4);
+    x.rows = (int4 *)take((size_t)T * 16);
     x.xp = (__nv_bfloat16 *)take((size_t)p.Tpad * in * 2);
     if (K) {
         x.ids = (int *)take((size_t)T * K * 4);
@@ -1097,32 +1144,34 @@ struct Call {
     cudaStream_t s;
 };
 
-// The targets, the rows that count and their hidden states; fills the common arguments.
-static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w, float *loss, float *lse,
-                  uint16_t *dX, int lddx, int cg, bool grad)
+// The targets, the rows that count and their hidden states; fills the common arguments. `k`
+// holds what one direction adds.
+static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w, Pack k, int cg, bool grad)
 {
     int st;
+    const float inv_temp = c.K ? 1.0f / c.temp : 1.0f;
     if (c.K) {
         st = launch_pdl(teacher_kernel, dim3(ceil_div(c.T, TEACHER_ROWS)), 32 * TEACHER_ROWS, 0, c.s, 1, w.ids, w.mass,
-                        w.count, w.entropy, c.ids, c.top, c.T, c.K, c.vocab, 1.0f / c.temp);
+                        w.count, w.entropy, c.ids, c.top, c.T, c.K, c.vocab, inv_temp);
         if (st) return st;
     }
     const int in_place = c.ldx % 8 == 0 && aligned(c.X, 16);
-    const int rows = std::max(8, ceil_div(c.T, PACK_BLOCKS));
-    st = launch_pdl(pack_kernel, dim3(ceil_div(c.T, rows)), 256, 0, c.s, 1, w.row_of, w.n_live, w.xp, loss, lse,
-                    reinterpret_cast<__nv_bfloat16 *>(dX), lddx, c.X, c.ldx, in_place, c.K ? nullptr : c.label, w.count,
-                    c.T, c.in, c.vocab, rows);
-    if (st) return st;
+    k.rows = w.rows; k.n_live = w.n_live; k.g_scale = w.g_scale;
+    k.xp = reinterpret_cast<uint16_t *>(w.xp);
+    k.X = c.X; k.label = c.label; k.count = w.count;
+    k.ldx = c.ldx; k.in_place = in_place;
+    k.T = c.T; k.in = c.in; k.vocab = c.vocab;
+    k.per = std::max(8, ceil_div(c.T, PACK_BLOCKS));
+    if ((st = launch_pdl(pack_kernel, dim3(ceil_div(c.T, k.per)), 256, 0, c.s, 1, k))) return st;
     *a = Args{};
     a->T = c.T; a->in = c.in;
-    a->n_live = w.n_live; a->row_of = w.row_of; a->Tpad = p.Tpad;
+    a->n_live = w.n_live; a->rows = w.rows; a->Tpad = p.Tpad;
     a->x_in_place = in_place;
     // the hidden states of a group stay in L2 while the vocabulary streams by: 48 MB of them
     a->group_z = (int)std::max<long long>(ROW_PAD, std::min<long long>(MAX_T, (48LL << 20) / (c.in * 2LL)));
-    a->ids = c.K ? w.ids : c.label;
-    a->mass = w.mass; a->count = w.count;
+    a->ids = w.ids; a->mass = w.mass;
     a->K = c.K ? c.K : 1;
-    a->inv_temp = c.K ? 1.0f / c.temp : 1.0f;
+    a->inv_temp = inv_temp;
     a->c = c.K ? (float)(1.4426950408889634 / (double)c.temp) : LOG2E;
     const void *x = in_place ? (const void *)c.X : (const void *)w.xp;
     const long long ldx = in_place ? c.ldx : c.in, xr = in_place ? c.T : p.Tpad;
@@ -1150,12 +1199,14 @@ static int forward(float *loss, float *lse, const Call &c, void *ws)
     layout(&w, static_cast<char *>(ws), p, c.T, c.in, c.K, false);
     Args a;
     Maps maps{};
-    if ((st = set_up(&a, &maps, c, p, w, loss, lse, nullptr, 0, 1, false))) return st;
+    Pack k{};
+    k.loss = loss; k.lse_out = lse;
+    if ((st = set_up(&a, &maps, c, p, w, k, 1, false))) return st;
     a.part = w.part; a.zt = w.zt;
     a.z = Piece{0, c.vocab, nullptr};
     if ((st = launch_head<LOSS, 1>(maps, a, sms, c.s))) return st;
-    return launch_pdl(join_kernel, dim3(p.Tpad / 32), 1024, 0, c.s, 1, loss, lse, w.part, 2 * p.tiles, p.Tpad, w.row_of,
-                      w.n_live, w.zt, w.mass, w.count, w.entropy, a.K, a.inv_temp);
+    return launch_pdl(join_kernel, dim3(p.Tpad / 32), 1024, 0, c.s, 1, loss, lse, w.part, 2 * p.tiles, p.Tpad, w.rows,
+                      w.n_live, w.zt, w.mass, w.entropy, a.K, a.inv_temp);
 }
 
 // Launch i forms piece i's dz beside the dX and dW of piece i - 1 (two dz buffers), so each
@@ -1169,8 +1220,10 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     layout(&w, static_cast<char *>(ws), p, c.T, c.in, c.K, true);
     Args a;
     Maps maps{};
-    if ((st = set_up(&a, &maps, c, p, w, nullptr, nullptr, dX, lddx, p.cg, true))) return st;
-    a.lse = lse; a.g = g;
+    Pack k{};
+    k.dX = reinterpret_cast<__nv_bfloat16 *>(dX); k.lddx = lddx; k.lse = lse; k.g = g;
+    if ((st = set_up(&a, &maps, c, p, w, k, p.cg, true))) return st;
+    a.g_scale = g ? w.g_scale : nullptr;
     a.acc = w.acc;
     a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);
