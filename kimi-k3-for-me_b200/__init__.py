@@ -631,7 +631,10 @@ def _scratch(ws, need, device):
 
 
 def _stream_of(stream, device):
-    return C.c_void_p((stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream)
+    if stream is not None:
+        return C.c_void_p(stream.cuda_stream)
+    # the current stream's handle without its Stream object (3 us of a 15 us call)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 @_on_device_of

@@ -102,7 +102,7 @@ __device__ __forceinline__ void join(Shared &s, uint32_t key, int id, uint32_t b
 
 // Trim the list to between K and K + SLACK of its best and raise the bar to them. Called by
 // the whole block with n = s.n read by all; leaves the list, n and the bar visible; returns n.
-__device__ __noinline__ int trim(Shared &s, int n, int K)
+__device__ __forceinline__ int trim(Shared &s, int n, int K)
 {
     uint64_t r[HOLD];
     uint32_t top = 0;
@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restric
     // quads lie on 16-byte boundaries; the first may start before the segment
     const int skew = (int)((reinterpret_cast<uintptr_t>(row + begin) & 15u) / 4);
     int n = 0;
-    for (int base = begin - skew; base < end; base += ROUND) {
-        float4 v[QUADS];
+    float4 v[QUADS];
+    auto fetch = [&](int base) {
 #pragma unroll
         for (int i = 0; i < QUADS; i++) {
             const int x = base + (i * THREADS + (int)threadIdx.x) * 4;
@@ -207,6 +207,9 @@ __global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restric
                 v[i].w = x + 3 >= begin && x + 3 < end ? row[x + 3] : NAN;
             }
         }
+    };
+    fetch(begin - skew);
+    for (int base = begin - skew; base < end; base += ROUND) {
         // fmaxf passes over NaN
         auto most = [](const float4 &q) { return fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)); };
         if (base + skew == begin) {
@@ -226,6 +229,7 @@ __global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restric
                     s.quad_id[p] = base + (i * THREADS + (int)threadIdx.x) * 4;
                 }
             }
+        if (base + ROUND < end) fetch(base + ROUND);   // on its way while the block sorts this one out
         __syncthreads();
         const int aside = s.n_quads;
         if (aside == 0) {                              // (read by all before anyone adds to it:
@@ -306,8 +310,9 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(int *__restrict__ idx, f
 
 static int segments(int rows, int vocab)
 {
-    // about four blocks an SM of 148, no segment shorter than a round
-    const int want = ceil_div(4 * 148, rows), most = ceil_div(vocab, ROUND);
+    // at most four blocks an SM (of 148), one wave, no segment shorter than a round: 576 rows in
+    // one segment each take 63 us (in two, before the loads ran ahead, 76 against 69)
+    const int want = 4 * 148 / rows, most = ceil_div(vocab, ROUND);
     return std::max(1, std::min(std::min(want, most), MAX_SEG));
 }
 
