@@ -588,11 +588,17 @@ def lm_head_argmax(X, W, ws=None, stream=None):
 
 # ------------------------------------------------------- fitting a draft head ------
 def _on_device_of(fn):
-    """Run a wrapper whose first argument is a CUDA tensor with that tensor's device current."""
+    """Run a wrapper whose first argument is a CUDA tensor with that tensor's device current,
+    and, given a stream, with that stream current: what the call allocates then belongs to it."""
     @functools.wraps(fn)
-    def call(x, *args, **kw):
+    def call(x, *args, stream=None, **kw):
         if not x.is_cuda:
             raise K3Error("expected a CUDA tensor")
+        if stream is not None:
+            if stream.device != x.device:
+                raise K3Error(f"the stream is on {stream.device}, the tensors on {x.device}")
+            with torch.cuda.stream(stream):
+                return fn(x, *args, **kw)
         if x.device.index == torch.cuda.current_device():
             return fn(x, *args, **kw)
         with torch.cuda.device(x.device):
@@ -630,18 +636,17 @@ def _scratch(ws, need, device):
     return ptr(ws), ws.numel(), ws     # the tensor is kept until the call is enqueued
 
 
-def _stream_of(stream, device):
-    if stream is not None:
-        return C.c_void_p(stream.cuda_stream)
-    # the current stream's handle without its Stream object (3 us of a 15 us call)
+def _raw_stream(device):
+    """The current stream's handle, without its Stream object (3 us of a 15 us call)."""
     return C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 @_on_device_of
-def topk_logits(logits, K, ws=None, stream=None):
+def topk_logits(logits, K, ws=None):
     """The K largest logits of each row of logits [rows][vocab]: (ids int32, values fp32)
     [rows][K], descending, equal values by ascending id, NaN never taken; a row that runs out
-    ends in id -1, -inf. The teacher entries of lm_head_distill."""
+    ends in id -1, -inf. The teacher entries of lm_head_distill. (This and the functions below also
+    take stream=, a torch.cuda.Stream to run on in place of the current one.)"""
     if logits.dim() != 2 or logits.dtype != torch.float32:
         raise K3Error(f"logits: expected fp32 [rows][vocab], got {logits.dtype} {tuple(logits.shape)}")
     (rows, vocab), dev = logits.shape, logits.device
@@ -650,13 +655,13 @@ def topk_logits(logits, K, ws=None, stream=None):
     if rows == 0:
         return idx, val
     wp, wn, ws = _scratch(ws, lib.k3gpu_topk_logits_workspace(rows, vocab, K), dev)
-    check(lib.k3gpu_topk_logits(ptr(idx), ptr(val), ptr(logits), rows, vocab, K, wp, wn, _stream_of(stream, dev)),
+    check(lib.k3gpu_topk_logits(ptr(idx), ptr(val), ptr(logits), rows, vocab, K, wp, wn, _raw_stream(dev)),
           "k3gpu_topk_logits")
     return idx, val
 
 
 @_on_device_of
-def lm_head_xent(X, W, label, ws=None, stream=None):
+def lm_head_xent(X, W, label, ws=None):
     """Softmax cross entropy of the lm_head product X [T][in] . W^T (bf16, the logits never
     written) against label int32 [T]: (loss, lse) fp32 [T]. A negative label is a row without a
     target: loss, lse and gradient 0."""
@@ -668,7 +673,7 @@ def lm_head_xent(X, W, label, ws=None, stream=None):
     if T == 0:
         return loss, lse
     wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
-    check(lib.k3gpu_lm_head_xent(ptr(loss), ptr(lse), xp, ldx, w, lab, n, vocab, T, wp, wn, _stream_of(stream, dev)),
+    check(lib.k3gpu_lm_head_xent(ptr(loss), ptr(lse), xp, ldx, w, lab, n, vocab, T, wp, wn, _raw_stream(dev)),
           "k3gpu_lm_head_xent")
     return loss, lse
 
@@ -682,7 +687,7 @@ def _grads(X, W, need_dx, need_dw):
 
 
 @_on_device_of
-def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
+def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=None):
     """The gradient of lm_head_xent from its lse and the loss's incoming gradient g fp32 [T]
     (None: 1): (dX [T][in], dW [vocab][in]) bf16, None where not needed (a frozen head)."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
@@ -693,12 +698,12 @@ def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=N
     if T and (need_dx or need_dw):
         wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
         check(lib.k3gpu_lm_head_xent_grad(ptr(dX), n, ptr(dW), gp, ls, xp, ldx, w, lab, n, vocab, T, wp, wn,
-                                          _stream_of(stream, dev)), "k3gpu_lm_head_xent_grad")
+                                          _raw_stream(dev)), "k3gpu_lm_head_xent_grad")
     return dX, dW
 
 
 @_on_device_of
-def lm_head_distill(X, W, ids, top, temp=1.0, ws=None, stream=None):
+def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
     """KL of the teacher's top logits (ids int32, top fp32 [T][K], e.g. topk_logits of its
     sweep) from the head's softmax, both at temperature temp: (loss, lse) fp32 [T]. Entries with a
     negative id or a logit of -inf are empty; a row without entries has loss, lse and
@@ -712,12 +717,12 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None, stream=None):
         return loss, lse
     wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
     check(lib.k3gpu_lm_head_distill(ptr(loss), ptr(lse), xp, ldx, w, ip, tp, K, float(temp), n, vocab, T, wp, wn,
-                                    _stream_of(stream, dev)), "k3gpu_lm_head_distill")
+                                    _raw_stream(dev)), "k3gpu_lm_head_distill")
     return loss, lse
 
 
 @_on_device_of
-def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, need_dw=True, ws=None, stream=None):
+def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, need_dw=True, ws=None):
     """The gradient of lm_head_distill (arguments and results as lm_head_xent_grad)."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
     dev, K = X.device, ids.shape[-1]
@@ -728,7 +733,7 @@ def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, ne
     if T and (need_dx or need_dw):
         wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
         check(lib.k3gpu_lm_head_distill_grad(ptr(dX), n, ptr(dW), gp, ls, xp, ldx, w, ip, tp, K, float(temp), n, vocab,
-                                             T, wp, wn, _stream_of(stream, dev)), "k3gpu_lm_head_distill_grad")
+                                             T, wp, wn, _raw_stream(dev)), "k3gpu_lm_head_distill_grad")
     return dX, dW
 
 

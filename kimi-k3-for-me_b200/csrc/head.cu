@@ -64,7 +64,7 @@ constexpr int Z_CHUNK = 16;                // 64-K steps of z summed in TMEM bef
 constexpr int GROUP_D = 16 * BM;           // rows of dX and dW walked together
 constexpr int MAXK = 128;
 constexpr int ROW_PAD = 2 * BM;            // packed rows end on a pair's tile
-constexpr int PACK_BLOCKS = 512, PACK_ROWS = 2048;
+constexpr int PACK_BLOCKS = 512, PACK_ROWS = 2048, PACK_COLS = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum Mode { LOSS, GRAD };
@@ -879,27 +879,32 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
     }
     __syncthreads();
     const bool copy = !(k.in_place && total == T);
-    for (int t = t0 + warp; t < t1; t += 8) {
-        const int p = place[t - t0];
-        if (p >= 0) {
-            if (!copy) continue;
+    // a warp takes a row's next PACK_COLS columns
+    const int parts = (in + PACK_COLS - 1) / PACK_COLS;
+    for (int w = warp; w < (t1 - t0) * parts; w += 8) {
+        const int t = t0 + w / parts, p = place[t - t0], c0 = w % parts * PACK_COLS, c1 = min(in, c0 + PACK_COLS);
+        if (p >= 0 && copy) {
             const uint16_t *x = k.X + (size_t)t * k.ldx;
+            uint16_t *o = k.xp + (size_t)p * in;
             if (k.in_place) {                      // rows 16-byte aligned
-#pragma unroll 4
-                for (int i = lane; i < in / 8; i += 32)
-                    reinterpret_cast<uint4 *>(k.xp + (size_t)p * in)[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
+#pragma unroll
+                for (int i = 0; i < PACK_COLS / 256; i++) {
+                    const int c = c0 + (i * 32 + lane) * 8;
+                    if (c < c1) *reinterpret_cast<uint4 *>(o + c) = __ldg(reinterpret_cast<const uint4 *>(x + c));
+                }
             } else {
-#pragma unroll 4
-                for (int i = lane; i < in; i += 32) k.xp[(size_t)p * in + i] = __ldg(x + i);
+#pragma unroll 8
+                for (int c = c0 + lane; c < c1; c += 32) o[c] = __ldg(x + c);
             }
-            continue;
         }
-        if (k.loss && lane == 0) {
-            k.loss[t] = 0.0f;
-            k.lse_out[t] = 0.0f;
+        if (p < 0) {
+            if (k.loss && c0 == 0 && lane == 0) {
+                k.loss[t] = 0.0f;
+                k.lse_out[t] = 0.0f;
+            }
+            if (k.dX)
+                for (int c = c0 + lane; c < c1; c += 32) k.dX[(size_t)t * k.lddx + c] = __float2bfloat16_rn(0.0f);
         }
-        if (k.dX)
-            for (int i = lane; i < in; i += 32) k.dX[(size_t)t * k.lddx + i] = __float2bfloat16_rn(0.0f);
     }
     if (copy)
         for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
@@ -1161,7 +1166,7 @@ static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w
     k.X = c.X; k.label = c.label; k.count = w.count;
     k.ldx = c.ldx; k.in_place = in_place;
     k.T = c.T; k.in = c.in; k.vocab = c.vocab;
-    k.per = std::max(8, ceil_div(c.T, PACK_BLOCKS));
+    k.per = ceil_div(c.T, PACK_BLOCKS);
     if ((st = launch_pdl(pack_kernel, dim3(ceil_div(c.T, k.per)), 256, 0, c.s, 1, k))) return st;
     *a = Args{};
     a->T = c.T; a->in = c.in;
@@ -1268,7 +1273,8 @@ static bool grads_ok(const uint16_t *dX, int lddx, const uint16_t *dW, int in)
 
 static bool teacher_ok(const int *ids, const float *top, int K, float temp)
 {
-    return ids && top && K > 0 && K <= MAXK && temp > 0.0f && isfinite(temp) && isfinite(1.0f / temp);
+    // (log2(e) / temp is what multiplies the logits)
+    return ids && top && K > 0 && K <= MAXK && temp > 0.0f && isfinite(temp) && isfinite((float)(1.4426950408889634 / temp));
 }
 
 }  // namespace head

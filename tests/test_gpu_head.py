@@ -369,3 +369,136 @@ def test_a_sweep_teaches_a_head(k3):
     want = formula(X, W, targets_xent(ids[:, 0], 1500), 1.0, g)
     for name in want:
         holds(name, got[name], want[name])
+
+
+def test_stream_argument(k3):
+    """stream=: the call and what it allocates belong to that stream; a stream of the caller's that
+    is still busy does not disturb it."""
+    X, W, g, gen = inputs(200, 256, 3000, 17)
+    label = torch.randint(-1, 3000, (200,), generator=gen, device="cuda").int()
+    want = xent_all(k3, X, W, label, g)
+    wi, wv = k3.topk_logits(X.float(), 9)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(4):
+        torch.randn(1 << 22, device="cuda").sort()                  # the current stream stays busy
+        loss, lse = k3.lm_head_xent(X, W, label, stream=side)
+        dX, dW = k3.lm_head_xent_grad(X, W, label, lse, g=g, stream=side)
+        got.append((loss, lse, dX, dW, *k3.topk_logits(X.float(), 9, stream=None)))
+    side.synchronize()
+    for loss, lse, dX, dW, ti, tv in got:
+        assert torch.equal(loss, want["loss"]) and torch.equal(lse, want["lse"])
+        assert torch.equal(dX, want["dX"]) and torch.equal(dW, want["dW"])
+        assert torch.equal(ti, wi) and torch.equal(tv, wv)
+
+
+def test_two_streams_at_once(k3):
+    """Two steps in flight together, each with its own workspace."""
+    a, b = inputs(300, 320, 4000, 18), inputs(310, 312, 4100, 19)
+    la = torch.randint(-1, 4000, (300,), generator=a[3], device="cuda").int()
+    lb = torch.randint(-1, 4100, (310,), generator=b[3], device="cuda").int()
+    wa, wb = xent_all(k3, a[0], a[1], la, a[2]), xent_all(k3, b[0], b[1], lb, b[2])
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    out = []
+    for _ in range(6):
+        with torch.cuda.stream(sa):
+            out.append((xent_all(k3, a[0], a[1], la, a[2]), wa))
+        with torch.cuda.stream(sb):
+            out.append((xent_all(k3, b[0], b[1], lb, b[2]), wb))
+    torch.cuda.synchronize()
+    for got, want in out:
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+    assert k3.device_status(0) == 0
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first call of each entry point is captured."""
+    code = (
+        "import sys; sys.path[:0] = [%r, %r]\n"
+        "import torch\n"
+        "from k3lib import load\n"
+        "k3 = load()\n"
+        "X = torch.randn((300, 128), device='cuda').bfloat16()\n"
+        "W = torch.randn((2000, 128), device='cuda').bfloat16()\n"
+        "ids = torch.randint(0, 2000, (300, 6), device='cuda').int()\n"
+        "top = torch.randn((300, 6), device='cuda')\n"
+        "lg = torch.randn((30, 20000), device='cuda')\n"
+        "torch.cuda.synchronize()\n"
+        "def run():\n"
+        "    t = k3.topk_logits(lg, 5)\n"
+        "    l = k3.lm_head_distill(X, W, ids, top)\n"
+        "    return (*t, *l, *k3.lm_head_distill_grad(X, W, ids, top, l[1]))\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    got = run()\n"
+        "g.replay()\n"
+        "for a, b in zip(got, run()):\n"
+        "    assert torch.equal(a, b)\n"
+        "print('same')\n" % (HERE, os.path.dirname(HERE)))
+    import subprocess
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+def test_far_offsets(k3):
+    """A head of 4.6e9 elements: offsets past 2^32 in W and dW. The logits of two rows in 64 bits,
+    a slice of the head at a time; dW at the first id, the targets and the last."""
+    n, vocab, T = 65536, 70001, 2
+    gen = torch.Generator(device="cuda").manual_seed(20)
+    X = torch.randn((T, n), generator=gen, device="cuda").bfloat16()
+    W = torch.empty((vocab, n), dtype=torch.bfloat16, device="cuda").normal_(0, 1 / math.sqrt(n), generator=gen)
+    label = torch.tensor([vocab - 1, 65537], dtype=torch.int32, device="cuda")
+    g = torch.tensor([0.75, -0.4], device="cuda")
+    got = xent_all(k3, X, W, label, g)
+    z, S = [], []
+    for v in range(0, vocab, 4096):
+        w = W[v:v + 4096].double()
+        z.append(X.double() @ w.T)
+        S.append(X.double().abs() @ w.abs().T)
+    z, S = torch.cat(z, 1), torch.cat(S, 1)
+    ez = ((n / 16 + 16) * 2.0 ** -23 * S).amax(1)
+    lse = torch.logsumexp(z, 1)
+    loss = lse - z.gather(1, label.long()[:, None])[:, 0]
+    mag = lse.abs() + z.abs().amax(1) + 1
+    holds("lse", got["lse"], (lse, ez + 2.0 ** -21 * mag))
+    holds("loss", got["loss"], (loss, 2 * ez + 2.0 ** -21 * mag))
+    p = (z - lse[:, None]).exp()
+    for v in (0, 32768, 65537, vocab - 1):
+        hit = (label == v).double()
+        dz = (p[:, v] - hit) * g.double()
+        b = dz.abs() * 2.0 ** -8 + g.double().abs() * (p[:, v] * (2 * ez + 2.0 ** -18 * mag) + hit * 2.0 ** -22)
+        want = dz @ X.double()
+        holds("dW", got["dW"][v], (want, b @ X.double().abs() + want.abs() * 2.0 ** -8 + 2.0 ** -18 * (dz.abs() @ X.double().abs())))
+
+
+def test_wrappers_refuse(k3):
+    X, W, g, gen = inputs(8, 64, 100, 21)
+    label = torch.zeros(8, dtype=torch.int32, device="cuda")
+    lse = torch.zeros(8, device="cuda")
+    ids, top = torch.zeros((8, 3), dtype=torch.int32, device="cuda"), torch.zeros((8, 3), device="cuda")
+    bad = [lambda: k3.lm_head_xent(X.float(), W, label), lambda: k3.lm_head_xent(X, W.half(), label),
+           lambda: k3.lm_head_xent(X[:, :56], W, label), lambda: k3.lm_head_xent(X, W, label.long()),
+           lambda: k3.lm_head_xent(X, W, label[:7]), lambda: k3.lm_head_xent(X, W, label.cpu()),
+           lambda: k3.lm_head_xent(X.cpu(), W, label), lambda: k3.lm_head_xent(X, W.cpu(), label),
+           lambda: k3.lm_head_xent(X, W.t().contiguous().t(), label), lambda: k3.lm_head_xent(X.t(), W, label),
+           lambda: k3.lm_head_xent(X[:1].expand(8, 64), W, label),
+           lambda: k3.lm_head_xent(X[:, :60], W[:, :60].contiguous(), label),           # not a multiple of 8
+           lambda: k3.lm_head_xent(X, W, label, ws=torch.empty(16, dtype=torch.uint8, device="cuda")),
+           lambda: k3.lm_head_xent(X, W, label, ws=torch.empty(1 << 20, device="cuda")),
+           lambda: k3.lm_head_xent_grad(X, W, label, lse.double()), lambda: k3.lm_head_xent_grad(X, W, label, lse[:4]),
+           lambda: k3.lm_head_xent_grad(X, W, label, lse, g=g.half()),
+           lambda: k3.lm_head_distill(X, W, ids, top[:, :2]), lambda: k3.lm_head_distill(X, W, ids.long(), top),
+           lambda: k3.lm_head_distill(X, W, ids, top, temp=0.0), lambda: k3.lm_head_distill(X, W, ids, top, temp=math.nan),
+           lambda: k3.lm_head_distill(X, W, ids.repeat(1, 43), top.repeat(1, 43)),      # 129 entries
+           lambda: k3.lm_head_distill_grad(X, W, ids, top, lse, temp=-1.0),
+           lambda: k3.topk_logits(X, 4), lambda: k3.topk_logits(top.t(), 2), lambda: k3.topk_logits(top, 129),
+           lambda: k3.topk_logits(top, 0), lambda: k3.topk_logits(top.cpu(), 2)]
+    for i, call in enumerate(bad):
+        with pytest.raises(k3.K3Error):
+            call()
+            pytest.fail(f"call {i} was taken")
+    k3.lm_head_xent_grad(X, W, label, lse, need_dx=False, need_dw=False)
+    assert k3.device_status(0) == 0

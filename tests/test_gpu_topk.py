@@ -108,3 +108,26 @@ def test_stream_and_graph(k3):
 def test_agrees_with_argmax(k3):
     a = torch.randn((40, 163840), device="cuda")
     assert torch.equal(k3.topk_logits(a, 1)[0][:, 0], k3.argmax(a))
+
+
+def test_far_offsets(k3):
+    """Rows past 2^31 elements from the first."""
+    rows, vocab, K = 14000, 163840, 16
+    a = torch.randn((rows, vocab), device="cuda")
+    idx, val = k3.topk_logits(a, K)
+    for r in (0, 13107, 13108, rows - 1):
+        wi, wv = want_of(a[r:r + 1].cpu().numpy(), K)
+        np.testing.assert_array_equal(idx[r:r + 1].cpu().numpy(), wi)
+        np.testing.assert_array_equal(val[r:r + 1].cpu().numpy(), wv)
+
+
+@pytest.mark.parametrize("K", [1, 100])
+def test_mostly_banned_rows(k3, K):
+    """Rows of which all but a few, or exactly K, or fewer than K ids are -inf, and rows of one value."""
+    n = 50000
+    rng = np.random.default_rng(K)
+    a = np.full((5, n), -np.inf, np.float32)
+    for r, m in enumerate((0, 1, K, K + 3)):
+        a[r, rng.permutation(n)[:m]] = rng.standard_normal(m)
+    a[4] = 1.5
+    check(k3, a, K)
