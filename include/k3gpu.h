@@ -428,8 +428,8 @@ int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, int ldx, cons
  * with g [T] the loss's incoming gradient (NULL: 1). dX [T][in] (row stride lddx) and dW
  * [vocab][in] (16-byte aligned) are bf16 bits, written whole, not added to; either may be
  * NULL (a frozen head needs no dW). dz is rounded to bf16 once; the sums are fp32. The
- * vocabulary is taken in pieces, so the workspace does not grow with T * vocab. Neither output
- * may overlap an input. */
+ * vocabulary is taken in pieces: of the size of the logits the workspace holds a sixty-fourth
+ * (the loss's running statistics). Neither output may overlap an input. */
 int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, const float *g,
                             const float *lse, const uint16_t *X, int ldx, const uint16_t *W,
                             const int *label, int in, int vocab, int T, void *workspace,

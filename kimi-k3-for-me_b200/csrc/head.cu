@@ -15,24 +15,38 @@
 // of its padding, say) reaches a sum. When every row counts, X is read in place.
 //
 // Forward: one pass over the vocabulary in 128 x 256 tiles; the epilogue keeps each row's
-// running maximum and sum of 2^(z c - max) over its tile half (c = log2(e)/temp) and picks
-// out the targets' z; a second kernel joins the halves' statistics per row in double.
+// maximum and sum of 2^(z c - max) over its tile half (c = log2(e)/temp) and picks out the
+// targets' z; a second kernel joins the halves' statistics per row.
 // Backward: the vocabulary in pieces. Per piece the tile products run again, the epilogue
-// turns z into dz from the saved lse and writes it as bf16 to the workspace [T][piece];
-// then one launch forms dX += dz W_piece (fp32 between pieces, bf16 at the end) and
-// dW_piece = dz^T X. dz is rounded to bf16 once, relative error 2^-9 an element, the size
-// of the outputs' own rounding and independent between elements; all sums are fp32.
+// turns z into dz from the saved lse and writes it as bf16 to the workspace [T][piece]; the
+// next launch forms dX += dz W_piece (fp32 between pieces, bf16 at the end) and
+// dW_piece = dz^T X, beside the dz of the piece after it (two buffers), so each launch has
+// several kinds of units to fill the SMs with. dz leaves out the factors common to all of
+// it (1/temp, the largest weight; the outputs get them in fp32) and is rounded to bf16
+// once: at most 2^-8 of an element, as much as the outputs' own rounding, independent
+// between elements. All sums are fp32.
 //
-// One persistent CTA per SM takes units of work from a counter (10 warps):
+// One persistent CTA per SM takes every n-th unit of work (10 warps):
 //   warp 0     TMA, a ring of 64-K stages: A 128 rows (16 KB), B 256 rows (32 KB)
 //   warp 1     one thread issues the MMAs (128 x 256 x 16) into one of two TMEM
 //              accumulators of 256 columns
 //   warps 2-9  epilogue of the finished accumulator while the next one fills: warp w reads
 //              the TMEM lane quarter w % 4, columns 128 ((w - 2) / 4) ..
+// In the backward of larger batches two CTAs of a cluster share a 256 x 256 unit
+// (cta_group::2): each loads its 128 rows of A and half of B.
 // The tensor core's fp32 sums are cut, not rounded, as they grow, an error with one sign; z
-// therefore leaves TMEM every 1024 of K and is summed in the epilogue's registers (for 7168
-// wide hidden states the loss is then 5.5e-7 from the 64-bit value and not 4.4e-6, at 0.3% of the time; the MMAs do not
-// wait, two accumulators alternate). dX and dW end in bf16 and stay in TMEM.
+// therefore leaves TMEM every 1024 of K and is summed in the epilogue's registers: over
+// 7168 wide hidden states the loss is 5.5e-7 from its 64-bit value, without that 4.4e-6, and
+// it costs 0.3% (the MMAs do not wait, two accumulators alternate). dX and dW end in bf16
+// and stay in TMEM.
+//
+// What bounds it: the tensor cores at the card's power limit. Alone, 2048 rows of 7168 over
+// 163,840 ids: the loss 3.12 ms (1.54 PFLOP/s, 0.91 of the measured burst rate), the gradient
+// 9.8 ms for the three products it runs (1.47), the tensor pipe 87-90% busy while the clock
+// falls to 1.33-1.44 GHz; back to back 14.4 ms together. A handful of rows is a weight
+// stream: 9 rows 0.44 ms, 5.3 TB/s of W.
+// Units dealt out by a counter instead of in turn cost 2-3% (neighbouring SMs then no longer
+// read the same W tile together), pairs in the forward 3%.
 // Every wait is bounded (a wait that gives up has waited seconds, longer than any copy in
 // flight takes); TMEM is freed on every exit path. No TMA multicast.
 #include <cuda_bf16.h>
@@ -61,7 +75,7 @@ template <int CG> struct Stage {
 };
 constexpr int HALF = BN / 2;               // columns an epilogue thread holds
 constexpr int Z_CHUNK = 16;                // 64-K steps of z summed in TMEM before they join the registers
-constexpr int GROUP_D = 16 * BM;           // rows of dX and dW walked together
+constexpr int GROUP_D = 16 * BM;           // rows of dX and dW walked together: 16 x 9 tiles in flight
 constexpr int MAXK = 128;
 constexpr int ROW_PAD = 2 * BM;            // packed rows end on a pair's tile
 constexpr int PACK_BLOCKS = 512, PACK_ROWS = 2048, PACK_COLS = 1024;
@@ -273,8 +287,8 @@ __device__ __forceinline__ void store64(uint32_t buf, const CUtensorMap *m, int 
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const uint4 o = word8(j);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) * 16))),
-                     "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w)
+        const uint32_t at = buf + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) * 16));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w)
                      : "memory");
     }
     fence_async_smem();
@@ -608,7 +622,9 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 if (failed) break;
                 if (MODE == LOSS) take(words_next, r_next);
                 if (MODE == LOSS) loss_epilogue(a, z, tg, r.x, row, live, col0);
-                else dz_epilogue(a, &maps.z_out, buf, z, tg, r.x, row0, lane, live, col0, __int_as_float(r.z), __int_as_float(r.w));
+                else
+                    dz_epilogue(a, &maps.z_out, buf, z, tg, r.x, row0, lane, live, col0, __int_as_float(r.z),
+                                __int_as_float(r.w));
                 __syncwarp();
                 if (MODE != LOSS) take(words_next, r_next);
             } else if (t.kind == DW) {
@@ -629,7 +645,9 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                     const int col = col0 + c0;
                     store64(buf, &maps.w_out, col, a.d.v0 + row0, col >= a.in || row0 >= a.d.vc, lane, [&](int j) {
                         const uint32_t *f = v[j >> 2] + 8 * (j & 3);
-                        auto pk = [&](int k) { return pack_bf16(__uint_as_float(f[k]) * scale, __uint_as_float(f[k + 1]) * scale); };
+                        auto pk = [&](int k) {
+                            return pack_bf16(__uint_as_float(f[k]) * scale, __uint_as_float(f[k + 1]) * scale);
+                        };
                         return make_uint4(pk(0), pk(2), pk(4), pk(6));
                     });
                 }
@@ -1048,7 +1066,8 @@ static Plan plan(int T, int in, int vocab)
     p.cg = 100LL * ceil_div(T, 2 * BM) * 2 < 107LL * ceil_div(T, BM) ? 2 : 1;
     p.Tpad = ceil_div(T, ROW_PAD) * ROW_PAD;
     p.tiles = ceil_div(vocab, BN);
-    // a piece's dz takes about 128 MB, at least eight tiles
+    // A piece's dz takes about 128 MB, at least eight tiles: with 64 MB the gradients take 1-4%
+    // longer (each launch ends unevenly), with 256 MB -1 to +2%.
     const long long tiles = std::max<long long>(8, (128LL << 20) / ((long long)p.Tpad * 2 * BN));
     p.piece = (int)std::min<long long>(tiles, p.tiles) * BN;
     p.pieces = ceil_div(vocab, p.piece);
@@ -1063,7 +1082,8 @@ static Plan plan(int T, int in, int vocab)
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (s > 1 && steps / s < 4) break;
         const int len = ceil_div(steps, s);
-        const double cost[3] = {len + (s > 1 || p.pieces > 1 ? 16.0 : 4.0), ceil_div(T, KB) + 4.0, ceil_div(in, KB) + 4.0};
+        const double cost[3] = {len + (s > 1 || p.pieces > 1 ? 16.0 : 4.0), ceil_div(T, KB) + 4.0,
+                                ceil_div(in, KB) + 4.0};
         const double t = busiest({(long long)rows * cols * s, n_w, 0}, cost, workers) +
                          (p.pieces - 1) * busiest({(long long)rows * cols * s, n_w, n_z}, cost, workers);
         if (s == 1 || t < 0.98 * best) {
@@ -1274,7 +1294,8 @@ static bool grads_ok(const uint16_t *dX, int lddx, const uint16_t *dW, int in)
 static bool teacher_ok(const int *ids, const float *top, int K, float temp)
 {
     // (log2(e) / temp is what multiplies the logits)
-    return ids && top && K > 0 && K <= MAXK && temp > 0.0f && isfinite(temp) && isfinite((float)(1.4426950408889634 / temp));
+    return ids && top && K > 0 && K <= MAXK && temp > 0.0f && isfinite(temp) &&
+           isfinite((float)(1.4426950408889634 / (double)temp));
 }
 
 }  // namespace head
