@@ -35,10 +35,10 @@
 // In the backward of larger batches two CTAs of a cluster share a 256 x 256 unit
 // (cta_group::2): each loads its 128 rows of A and half of B.
 // The tensor core's fp32 sums are cut, not rounded, as they grow, an error with one sign; z
-// therefore leaves TMEM every 1024 of K and is summed in the epilogue's registers: over
-// 7168 wide hidden states the loss is 5.5e-7 from its 64-bit value, without that 4.4e-6, and
-// it costs 0.3% (the MMAs do not wait, two accumulators alternate). dX and dW end in bf16
-// and stay in TMEM.
+// therefore leaves TMEM every 512 of K (256 for a weight stream; 2048 in the backward, where
+// dz's rounding covers it) and is summed in the epilogue's registers: over 7168 wide hidden
+// states the loss is 2.5e-7 from its 64-bit value, without that 4.4e-6, and it costs 0.8%
+// (the MMAs do not wait, two accumulators alternate). dX and dW end in bf16 and stay in TMEM.
 //
 // What bounds it: the tensor cores at the card's power limit. Alone, 2048 rows of 7168 over
 // 163,840 ids: the loss 3.12 ms (1.54 PFLOP/s, 0.91 of the measured burst rate), the gradient
@@ -74,7 +74,6 @@ template <int CG> struct Stage {
     static constexpr int B_COLS = BN / CG, BYTES = A_BYTES + B_COLS * KB * 2, N = RING / BYTES;
 };
 constexpr int HALF = BN / 2;               // columns an epilogue thread holds
-constexpr int Z_CHUNK = 16;                // 64-K steps of z summed in TMEM before they join the registers
 constexpr int GROUP_D = 16 * BM;           // rows of dX and dW walked together: 16 x 9 tiles in flight
 constexpr int MAXK = 128;
 constexpr int ROW_PAD = 2 * BM;            // packed rows end on a pair's tile
@@ -101,6 +100,7 @@ struct Args {
     const float *mass;
     int K;
     float c;                    // log2(e) / temp
+    int chunk;                  // 64-K steps of z summed in TMEM before they join the registers
     Piece z;                    // vc = 0: no z units in this launch
     // LOSS
     float2 *part;               // [2 * vocabulary tiles][Tpad] (max, sum), base 2
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 const bool b_mn = MODE == GRAD && t.kind != Z, a_mn = MODE == GRAD && t.kind == DW;
                 const uint32_t idesc = (bf16_idesc(BN, b_mn) + ((uint32_t)(CG - 1) << 27)) | (a_mn ? (1u << 15) : 0u);
                 const uint32_t da = a_mn ? 2048u >> 4 : 32u >> 4, db = b_mn ? 2048u >> 4 : 32u >> 4;
-                const int chunk = b_mn ? t.steps : Z_CHUNK;
+                const int chunk = b_mn ? t.steps : a.chunk;
                 for (int ks = 0; ks < t.steps && !failed; use++) {
                     const int d = use & 1, end = min(t.steps, ks + chunk);
                     if (!bar_wait(s_addr(&b_free[d]), (uint32_t)((use >> 1) & 1) ^ 1u)) { failed = true; break; }
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 tmem_wait_ld();
                 release();
 #pragma unroll 1
-                for (int ks = Z_CHUNK; ks < t.steps; ks += Z_CHUNK) {
+                for (int ks = a.chunk; ks < t.steps; ks += a.chunk) {
                     if (!finished()) { failed = true; break; }
 #pragma unroll
                     for (int c0 = 0; c0 < HALF; c0 += 16) {
@@ -1229,6 +1229,7 @@ static int forward(float *loss, float *lse, const Call &c, void *ws)
     if ((st = set_up(&a, &maps, c, p, w, k, 1, false))) return st;
     a.part = w.part; a.zt = w.zt;
     a.z = Piece{0, c.vocab, nullptr};
+    a.chunk = c.T <= BM ? 4 : 8;           // (a weight stream leaves the time for it)
     if ((st = launch_head<LOSS, 1>(maps, a, sms, c.s))) return st;
     return launch_pdl(join_kernel, dim3(p.Tpad / 32), 1024, 0, c.s, 1, loss, lse, w.part, 2 * p.tiles, p.Tpad, w.rows,
                       w.n_live, w.zt, w.mass, w.entropy, a.K, a.inv_temp);
@@ -1249,6 +1250,7 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     k.dX = reinterpret_cast<__nv_bfloat16 *>(dX); k.lddx = lddx; k.lse = lse; k.g = g;
     if ((st = set_up(&a, &maps, c, p, w, k, p.cg, true))) return st;
     a.g_scale = g ? w.g_scale : nullptr;
+    a.chunk = 32;                          // what it adds to p is far below dz's rounding
     a.acc = w.acc;
     a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);
