@@ -409,7 +409,7 @@ int k3gpu_topk_logits(int *idx, float *val, const float *logits, int rows, int v
 
 /* The losses of a draft head over the lm_head product (k3gpu_lm_head_argmax's form: the
  * [T][vocab] logits are never written). X [T][in] bf16 bits, row stride ldx elements (any
- * ldx >= in; rows that are 16-byte aligned are read in place), W [vocab][in] bf16 bits,
+ * ldx >= in; rows on 16-byte boundaries are best), W [vocab][in] bf16 bits,
  * 16-byte aligned; z = X W^T with exact products and fp32 sums.
  * Limits: in % 8 == 0, in <= 65536, vocab <= 2^24, T <= 2^20; the workspace is 256-byte
  * aligned, the same for a loss and its gradient. The reference has no training code; these

@@ -44,7 +44,7 @@
 // 163,840 ids: the loss 3.12 ms (1.54 PFLOP/s, 0.91 of the measured burst rate), the gradient
 // 9.8 ms for the three products it runs (1.47), the tensor pipe 87-90% busy while the clock
 // falls to 1.33-1.44 GHz; back to back 14.4 ms together. A handful of rows is a weight
-// stream: 9 rows 0.44 ms, 5.3 TB/s of W.
+// stream: 9 rows 0.39 ms, 6.0 TB/s of W.
 // Units dealt out by a counter instead of in turn cost 2-3% (neighbouring SMs then no longer
 // read the same W tile together), pairs in the forward 3%.
 // Every wait is bounded (a wait that gives up has waited seconds, longer than any copy in
@@ -824,7 +824,8 @@ __global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *__restr
 // their places and writes zeros for the others' outputs. Each block takes `per` rows and
 // counts the live ones before them itself (T * 4 bytes from L2, at most PACK_BLOCKS blocks),
 // so one launch does it. When every row counts and X can be read in place nothing is copied;
-// else the rows from the last packed one to the end of its tile become zeros.
+// else the rows from the last packed one to the end of its K step become zeros: dW sums over
+// them. (What z's tiles read past those is of rows that do not count.)
 // The weights are divided by the largest of them (*g_scale): a mean's common 1 / n then
 // rounds nothing when dz becomes bf16. (Where the largest is 0 or not finite, by 1.)
 struct Pack {
@@ -837,7 +838,8 @@ struct Pack {
     const float *lse, *g;
     const uint16_t *X;
     const int *label, *count;          // one of them
-    int lddx, ldx, in_place, T, in, vocab, per;
+    int lddx, ldx, vec, in_place;      // vec: X's rows lie on 16 bytes
+    int T, in, vocab, per;
 };
 
 __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
@@ -904,7 +906,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
         if (p >= 0 && copy) {
             const uint16_t *x = k.X + (size_t)t * k.ldx;
             uint16_t *o = k.xp + (size_t)p * in;
-            if (k.in_place) {                      // rows 16-byte aligned
+            if (k.vec) {
 #pragma unroll
                 for (int i = 0; i < PACK_COLS / 256; i++) {
                     const int c = c0 + (i * 32 + lane) * 8;
@@ -925,8 +927,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
         }
     }
     if (copy)
-        for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
-             p += (int)gridDim.x * 8)
+        for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + KB - 1) / KB * KB; p += (int)gridDim.x * 8)
             for (int i = lane; i < in / 8; i += 32)
                 reinterpret_cast<uint4 *>(k.xp + (size_t)p * in)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
@@ -1180,11 +1181,14 @@ static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w
                         w.count, w.entropy, c.ids, c.top, c.T, c.K, c.vocab, inv_temp);
         if (st) return st;
     }
-    const int in_place = c.ldx % 8 == 0 && aligned(c.X, 16);
+    // Read in place where TMA can, and where the rows span 128 KB: with a smaller tensor map the
+    // weight stream beside it is a fifth slower (9 rows of 7168 over 163,840 ids 490 us, 10 rows
+    // 400, the 9 copied to a map of 256 rows 411; the same step at 12 to 16 rows of 4096).
+    const int vec = c.ldx % 8 == 0 && aligned(c.X, 16), in_place = vec && (long long)c.T * c.ldx >= (64 << 10);
     k.rows = w.rows; k.n_live = w.n_live; k.g_scale = w.g_scale;
     k.xp = reinterpret_cast<uint16_t *>(w.xp);
     k.X = c.X; k.label = c.label; k.count = w.count;
-    k.ldx = c.ldx; k.in_place = in_place;
+    k.ldx = c.ldx; k.vec = vec; k.in_place = in_place;
     k.T = c.T; k.in = c.in; k.vocab = c.vocab;
     k.per = ceil_div(c.T, PACK_BLOCKS);
     if ((st = launch_pdl(pack_kernel, dim3(ceil_div(c.T, k.per)), 256, 0, c.s, 1, k))) return st;
