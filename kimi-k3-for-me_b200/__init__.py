@@ -607,38 +607,45 @@ def _on_device_of(fn):
 
 
 def _arg(name, t, device, dtype, shape):
-    """Device pointer of a contiguous tensor, checked against what the call needs."""
-    if t.device != device or t.dtype != dtype or t.shape != shape:
-        raise K3Error(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on "
-                      f"{t.device}")
-    return ptr(t)
+    """Address of a contiguous tensor, checked against what the call needs."""
+    if t.device != device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise K3Error(f"{name}: expected contiguous {dtype} {tuple(shape)} on {device}, got {t.dtype} "
+                      f"{tuple(t.shape)} (strides {t.stride()}) on {t.device}")
+    return t.data_ptr()
+
+
+_BF16_BITS = {torch.bfloat16, torch.int16, torch.uint16}
 
 
 def _head_args(X, W):
-    """(X pointer, row stride, W pointer, width, vocab, T) of a draft-head loss, checked."""
+    """(X address, row stride, W address, width, vocab, T) of a draft-head loss, checked."""
     for name, t in (("X", X), ("W", W)):
-        if t.dim() != 2 or t.dtype not in (torch.bfloat16, torch.int16, torch.uint16):
+        if t.dim() != 2 or t.dtype not in _BF16_BITS:
             raise K3Error(f"{name}: expected a 2-D tensor of bfloat16 (or its bits), got {t.dtype} {tuple(t.shape)}")
     (T, n), (vocab, m) = X.shape, W.shape
     if n != m or X.device != W.device:
         raise K3Error(f"X {tuple(X.shape)} on {X.device} and W {tuple(W.shape)} on {W.device} do not match")
-    ldx = X.stride(0) if T > 1 else n
-    if X.stride(1) != 1 or ldx < n:
+    ldx, step = X.stride()
+    if T <= 1:
+        ldx = n
+    if step != 1 or ldx < n:
         raise K3Error("X: expected rows of consecutive elements that do not overlap")
-    return C.c_void_p(X.data_ptr()), ldx, ptr(W), n, vocab, T
+    if not W.is_contiguous():
+        raise K3Error("W: expected a contiguous tensor")
+    return X.data_ptr(), ldx, W.data_ptr(), n, vocab, T
 
 
 def _scratch(ws, need, device):
     if ws is None:
-        ws = workspace(need, device)
-    elif ws.device != device or ws.dtype != torch.uint8:
-        raise K3Error(f"workspace: expected uint8 on {device}, got {ws.dtype} on {ws.device}")
-    return ptr(ws), ws.numel(), ws     # the tensor is kept until the call is enqueued
+        return torch.empty(max(need, 256), dtype=torch.uint8, device=device)
+    if ws.device != device or ws.dtype != torch.uint8 or not ws.is_contiguous():
+        raise K3Error(f"workspace: expected contiguous uint8 on {device}, got {ws.dtype} on {ws.device}")
+    return ws
 
 
 def _raw_stream(device):
     """The current stream's handle, without its Stream object (3 us of a 15 us call)."""
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 @_on_device_of
@@ -647,16 +654,16 @@ def topk_logits(logits, K, ws=None):
     [rows][K], descending, equal values by ascending id, NaN never taken; a row that runs out
     ends in id -1, -inf. The teacher entries of lm_head_distill. (This and the functions below also
     take stream=, a torch.cuda.Stream to run on in place of the current one.)"""
-    if logits.dim() != 2 or logits.dtype != torch.float32:
-        raise K3Error(f"logits: expected fp32 [rows][vocab], got {logits.dtype} {tuple(logits.shape)}")
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
+        raise K3Error(f"logits: expected contiguous fp32 [rows][vocab], got {logits.dtype} {tuple(logits.shape)}")
     (rows, vocab), dev = logits.shape, logits.device
-    idx = torch.empty((rows, K), dtype=torch.int32, device=dev)
-    val = torch.empty((rows, K), dtype=torch.float32, device=dev)
+    idx = torch.empty(rows, K, dtype=torch.int32, device=dev)
+    val = torch.empty(rows, K, dtype=torch.float32, device=dev)
     if rows == 0:
         return idx, val
-    wp, wn, ws = _scratch(ws, lib.k3gpu_topk_logits_workspace(rows, vocab, K), dev)
-    check(lib.k3gpu_topk_logits(ptr(idx), ptr(val), ptr(logits), rows, vocab, K, wp, wn, _raw_stream(dev)),
-          "k3gpu_topk_logits")
+    ws = _scratch(ws, lib.k3gpu_topk_logits_workspace(rows, vocab, K), dev)
+    check(lib.k3gpu_topk_logits(idx.data_ptr(), val.data_ptr(), logits.data_ptr(), rows, vocab, K, ws.data_ptr(),
+                                ws.numel(), _raw_stream(dev)), "k3gpu_topk_logits")
     return idx, val
 
 
@@ -672,18 +679,19 @@ def lm_head_xent(X, W, label, ws=None):
     lse = torch.empty(T, dtype=torch.float32, device=dev)
     if T == 0:
         return loss, lse
-    wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
-    check(lib.k3gpu_lm_head_xent(ptr(loss), ptr(lse), xp, ldx, w, lab, n, vocab, T, wp, wn, _raw_stream(dev)),
-          "k3gpu_lm_head_xent")
+    ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
+    check(lib.k3gpu_lm_head_xent(loss.data_ptr(), lse.data_ptr(), xp, ldx, w, lab, n, vocab, T, ws.data_ptr(),
+                                 ws.numel(), _raw_stream(dev)), "k3gpu_lm_head_xent")
     return loss, lse
 
 
 def _grads(X, W, need_dx, need_dw):
-    dX = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device) if need_dx else None
-    dW = torch.empty(W.shape, dtype=torch.bfloat16, device=X.device) if need_dw else None
+    """(dX, its address, dW, its address), None where not needed."""
+    dX = torch.empty(X.shape[0], X.shape[1], dtype=torch.bfloat16, device=X.device) if need_dx else None
+    dW = torch.empty(W.shape[0], W.shape[1], dtype=torch.bfloat16, device=X.device) if need_dw else None
     if X.shape[0] == 0 and need_dw:
         dW.zero_()
-    return dX, dW
+    return dX, dX.data_ptr() if need_dx else None, dW, dW.data_ptr() if need_dw else None
 
 
 @_on_device_of
@@ -694,10 +702,10 @@ def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=N
     dev = X.device
     lab, ls = _arg("label", label, dev, torch.int32, (T,)), _arg("lse", lse, dev, torch.float32, (T,))
     gp = _arg("g", g, dev, torch.float32, (T,)) if g is not None else None
-    dX, dW = _grads(X, W, need_dx, need_dw)
+    dX, dx, dW, dw = _grads(X, W, need_dx, need_dw)
     if T and (need_dx or need_dw):
-        wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
-        check(lib.k3gpu_lm_head_xent_grad(ptr(dX), n, ptr(dW), gp, ls, xp, ldx, w, lab, n, vocab, T, wp, wn,
+        ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
+        check(lib.k3gpu_lm_head_xent_grad(dx, n, dw, gp, ls, xp, ldx, w, lab, n, vocab, T, ws.data_ptr(), ws.numel(),
                                           _raw_stream(dev)), "k3gpu_lm_head_xent_grad")
     return dX, dW
 
@@ -715,9 +723,9 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
     lse = torch.empty(T, dtype=torch.float32, device=dev)
     if T == 0:
         return loss, lse
-    wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
-    check(lib.k3gpu_lm_head_distill(ptr(loss), ptr(lse), xp, ldx, w, ip, tp, K, float(temp), n, vocab, T, wp, wn,
-                                    _raw_stream(dev)), "k3gpu_lm_head_distill")
+    ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
+    check(lib.k3gpu_lm_head_distill(loss.data_ptr(), lse.data_ptr(), xp, ldx, w, ip, tp, K, float(temp), n, vocab, T,
+                                    ws.data_ptr(), ws.numel(), _raw_stream(dev)), "k3gpu_lm_head_distill")
     return loss, lse
 
 
@@ -729,11 +737,12 @@ def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, ne
     ip, tp = _arg("ids", ids, dev, torch.int32, (T, K)), _arg("top", top, dev, torch.float32, (T, K))
     ls = _arg("lse", lse, dev, torch.float32, (T,))
     gp = _arg("g", g, dev, torch.float32, (T,)) if g is not None else None
-    dX, dW = _grads(X, W, need_dx, need_dw)
+    dX, dx, dW, dw = _grads(X, W, need_dx, need_dw)
     if T and (need_dx or need_dw):
-        wp, wn, ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
-        check(lib.k3gpu_lm_head_distill_grad(ptr(dX), n, ptr(dW), gp, ls, xp, ldx, w, ip, tp, K, float(temp), n, vocab,
-                                             T, wp, wn, _raw_stream(dev)), "k3gpu_lm_head_distill_grad")
+        ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
+        check(lib.k3gpu_lm_head_distill_grad(dx, n, dw, gp, ls, xp, ldx, w, ip, tp, K, float(temp), n, vocab, T,
+                                             ws.data_ptr(), ws.numel(), _raw_stream(dev)),
+              "k3gpu_lm_head_distill_grad")
     return dX, dW
 
 
