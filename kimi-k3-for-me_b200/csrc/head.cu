@@ -22,7 +22,7 @@
 // next launch forms dX += dz W_piece (fp32 between pieces, bf16 at the end) and
 // dW_piece = dz^T X, beside the dz of the piece after it (two buffers), so each launch has
 // several kinds of units to fill the SMs with. dz leaves out the factors common to all of
-// it (1/temp, the largest weight; the outputs get them in fp32) and is rounded to bf16
+// it (1/temp, the largest weight's mantissa; the outputs get them in fp32) and is rounded to bf16
 // once: at most 2^-8 of an element, as much as the outputs' own rounding, independent
 // between elements. All sums are fp32.
 //
@@ -826,8 +826,9 @@ __global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *__restr
 // so one launch does it. When every row counts and X can be read in place nothing is copied;
 // else the rows from the last packed one to the end of its K step become zeros: dW sums over
 // them. (What z's tiles read past those is of rows that do not count.)
-// The weights are divided by the largest of them (*g_scale): a mean's common 1 / n then
-// rounds nothing when dz becomes bf16. (Where the largest is 0 or not finite, by 1.)
+// The weights are divided by the mantissa of the largest of them (*g_scale): a mean's common
+// 1 / n is then a power of two, which rounds nothing when dz becomes bf16, and weights of
+// any ratio keep their range. (Where the largest is 0 or not finite, by 1.)
 struct Pack {
     int4 *rows;
     int *n_live;
@@ -877,7 +878,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
         total += red[1][w];
         g_max = fmaxf(g_max, red_g[w]);
     }
-    const float g_scale = k.g && g_max > 0.0f && g_max < INFINITY ? g_max : 1.0f;
+    // the mantissa in [1, 2); of an extreme weight all of it
+    float g_scale = 1.0f;
+    if (k.g && g_max > 0.0f && g_max < INFINITY) {
+        const unsigned bits = __float_as_uint(g_max), e = bits >> 23;
+        g_scale = e >= 27 && e <= 227 ? __uint_as_float((bits & 0x7FFFFFu) | 0x3F800000u) : g_max;
+    }
     if (warp == 0) {
         for (int b = t0; b < t1; b += 32) {
             const int t = b + lane;
