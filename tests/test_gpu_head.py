@@ -530,3 +530,25 @@ def test_wrappers_refuse(k3):
             pytest.fail(f"call {i} was taken")
     k3.lm_head_xent_grad(X, W, label, lse, need_dx=False, need_dw=False)
     assert k3.device_status(0) == 0
+
+
+def test_a_model_sweep_teaches_a_head(k3, tmp_path):
+    """From the whole model's verify sweep: the top entries of its logits buffer (the first of them
+    the sweep's own argmax), and a draft head's step on them."""
+    model = k3.Model.from_checkpoint(k3._sibling("synth").write_checkpoint(str(tmp_path), seed=0), B=1, max_T=8,
+                                     kv_cap=64)
+    prompt = torch.randint(0, model.vocab, (1, 6), device="cuda").int()
+    model.prefill(prompt)
+    arg, logits = model.verify(torch.randint(0, model.vocab, (1, 8), device="cuda").int())
+    flat = logits.view(8, model.vocab)
+    ids, top = k3.topk_logits(flat, 16)
+    assert torch.equal(ids[:, 0], arg[0])
+    want = flat.double().cpu().sort(dim=1, descending=True, stable=True)
+    assert torch.equal(ids.cpu().long(), want.indices[:, :16])
+    assert torch.equal(top.cpu().double(), want.values[:, :16])
+    X, W, g, _ = inputs(8, 128, model.vocab, 23)
+    got = distill_all(k3, X, W, ids, top, 1.0, g)
+    bounds = formula(X, W, targets_distill(ids, top, 1.0, model.vocab), 1.0, g)
+    model.close()
+    for name in bounds:
+        holds(name, got[name], bounds[name])
