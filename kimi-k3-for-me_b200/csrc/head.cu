@@ -35,10 +35,10 @@
 // In the backward of larger batches two CTAs of a cluster share a 256 x 256 unit
 // (cta_group::2): each loads its 128 rows of A and half of B.
 // The tensor core's fp32 sums are cut, not rounded, as they grow, an error with one sign; z
-// therefore leaves TMEM every 512 of K (256 for a weight stream; 2048 in the backward, where
-// dz's rounding covers it) and is summed in the epilogue's registers: over 7168 wide hidden
-// states the loss is 2.5e-7 from its 64-bit value, without that 4.4e-6, and it costs 0.8%
-// (the MMAs do not wait, two accumulators alternate). dX and dW end in bf16 and stay in TMEM.
+// therefore leaves TMEM every 1024 of K (256 for a weight stream) and is summed in the
+// epilogue's registers: over 7168 wide hidden states the loss is 5.6e-7 from its 64-bit value,
+// without that 4.4e-6, and it costs 0.3% (the MMAs do not wait, two accumulators alternate;
+// every 512: 2.6e-7 and 1.5%). dX and dW end in bf16 and stay in TMEM.
 //
 // What bounds it: the tensor cores at the card's power limit. Alone, 2048 rows of 7168 over
 // 163,840 ids: the loss 3.12 ms (1.54 PFLOP/s, 0.91 of the measured burst rate), the gradient
@@ -363,10 +363,12 @@ __device__ __forceinline__ void loss_epilogue(const Args &a, float (&z)[HALF], R
 #pragma unroll
     for (int j = 0; j < HALF; j += 2) mx[(j >> 1) & 3] = fmaxf(mx[(j >> 1) & 3], fmaxf(z[j], z[j + 1]));
     const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.c, ref = m == -INFINITY ? 0.0f : m;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < HALF; j++) s[j & 3] += ex2(fmaf(z[j], a.c, -ref));
-    if (live) a.part[(size_t)(col0 / HALF) * a.Tpad + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
+    for (int j = 0; j < HALF; j++) s[j & 7] += ex2(fmaf(z[j], a.c, -ref));
+    if (live)
+        a.part[(size_t)(col0 / HALF) * a.Tpad + row] =
+            make_float2(m, ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])));
 }
 
 __device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *out, uint32_t buf, float (&z)[HALF],
@@ -943,7 +945,7 @@ __global__ void __launch_bounds__(1024) join_kernel(float *__restrict__ loss, fl
                                                     const float2 *__restrict__ part, int halves, int Tpad,
                                                     const int4 *__restrict__ rows, const int *__restrict__ n_live,
                                                     const float *__restrict__ zt, const float *__restrict__ mass,
-                                                    const float *__restrict__ entropy, int K, float inv_temp)
+                                                    const float *__restrict__ entropy, int K, float c)
 {
     __shared__ float sm[32][33];
     __shared__ float ss[32][33];
@@ -993,9 +995,11 @@ __global__ void __launch_bounds__(1024) join_kernel(float *__restrict__ loss, fl
         zq += __shfl_xor_sync(0xffffffffu, zq, o);
     }
     if (r == 0) {
-        const double l = ((double)ref + log2(S)) * 0.69314718055994530942;
-        lse[t] = (float)l;
-        loss[t] = (float)(l - zq * (double)inv_temp + (entropy ? (double)entropy[t] : 0.0));
+        // in base 2 until the difference is taken: a sure row's loss is small against both, and
+        // the targets' z meet the sum's with the factor that it has
+        const double l = (double)ref + log2(S), ln2 = 0.69314718055994530942;
+        lse[t] = (float)(l * ln2);
+        loss[t] = (float)((l - zq * (double)c) * ln2 + (entropy ? (double)entropy[t] : 0.0));
     }
 }
 
@@ -1206,6 +1210,8 @@ static int set_up(Args *a, Maps *maps, const Call &c, const Plan &p, const Ws &w
     a->group_z = (int)std::max<long long>(ROW_PAD, std::min<long long>(MAX_T, (48LL << 20) / (c.in * 2LL)));
     a->ids = w.ids; a->mass = w.mass;
     a->K = c.K ? c.K : 1;
+    // the same in both directions: where p is near 1, p - 1 lives on z and lse agreeing
+    a->chunk = c.T <= BM ? 4 : 16;         // (a weight stream leaves the time for it)
     a->inv_temp = inv_temp;
     a->c = c.K ? (float)(1.4426950408889634 / (double)c.temp) : LOG2E;
     const void *x = in_place ? (const void *)c.X : (const void *)w.xp;
@@ -1239,10 +1245,9 @@ static int forward(float *loss, float *lse, const Call &c, void *ws)
     if ((st = set_up(&a, &maps, c, p, w, k, 1, false))) return st;
     a.part = w.part; a.zt = w.zt;
     a.z = Piece{0, c.vocab, nullptr};
-    a.chunk = c.T <= BM ? 4 : 8;           // (a weight stream leaves the time for it)
     if ((st = launch_head<LOSS, 1>(maps, a, sms, c.s))) return st;
     return launch_pdl(join_kernel, dim3(p.Tpad / 32), 1024, 0, c.s, 1, loss, lse, w.part, 2 * p.tiles, p.Tpad, w.rows,
-                      w.n_live, w.zt, w.mass, w.entropy, a.K, a.inv_temp);
+                      w.n_live, w.zt, w.mass, w.entropy, a.K, a.c);
 }
 
 // Launch i forms piece i's dz beside the dX and dW of piece i - 1 (two dz buffers), so each
@@ -1260,7 +1265,6 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     k.dX = reinterpret_cast<__nv_bfloat16 *>(dX); k.lddx = lddx; k.lse = lse; k.g = g;
     if ((st = set_up(&a, &maps, c, p, w, k, p.cg, true))) return st;
     a.g_scale = g ? w.g_scale : nullptr;
-    a.chunk = 32;                          // what it adds to p is far below dz's rounding
     a.acc = w.acc;
     a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);

@@ -299,6 +299,38 @@ def test_gradient_against_differences(k3):
         assert ((got - want).abs() <= g.double().abs() * (move ** 3 * d * d / 6 + loss_err + grad_err)).all()
 
 
+@pytest.mark.parametrize("T,n,vocab", [(70, 1024, 2000), (200, 3200, 900), (300, 7168, 5000)])
+def test_sure_rows(k3, T, n, vocab):
+    """Rows that are nearly right (p of the label 0.99 to 0.9999): the loss and p - 1 are small
+    differences. The same z stands on both sides of them, so what is left is
+      loss  2 (1 - p) ez, and the fp32 sum of 2^(z - max): 32 additions beside a 1, 2^-19
+      p     the fp32 lse and its product with log2 e, 2^-22 |lse|, and the exp2, 2^-22 =: d
+      dX    a row's norm: d (|W_label| + sum p |W|), and the roundings of dz and dX."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    W = (torch.randn((vocab, n), generator=gen, device="cuda") * (1.7 / math.sqrt(n))).bfloat16()
+    label = torch.randint(0, vocab, (T,), generator=gen, device="cuda").int()
+    X = torch.randn((T, n), generator=gen, device="cuda")
+    Wl = W[label.long()].float()
+    lean = torch.empty(T, device="cuda").uniform_(5, 9, generator=gen) + math.log(vocab)
+    X = (X + Wl * ((lean - (X * Wl).sum(1)) / (Wl * Wl).sum(1))[:, None]).bfloat16()
+    Xd, Wd, at = X.double(), W.double(), label.long()[:, None]
+    z = Xd @ Wd.T
+    lse, zl = torch.logsumexp(z, 1), z.gather(1, at)[:, 0]
+    rest = torch.logsumexp(z.scatter(1, at, -math.inf), 1) - zl
+    loss = torch.log1p(rest.exp())
+    miss = -torch.expm1(-loss)                                        # 1 - p
+    assert 1e-5 < float(miss.min()) and float(miss.median()) < 0.02
+    dz = (z - lse[:, None]).exp().scatter(1, at, -miss[:, None])
+    dX = dz @ Wd
+    got, got_lse = k3.lm_head_xent(X, W, label)
+    grad, _ = k3.lm_head_xent_grad(X, W, label, got_lse, need_dw=False)
+    ez = ((n / 16 + 16) * 2.0 ** -23 * (Xd.abs() @ Wd.abs().T)).amax(1)
+    assert bool(((got.double() - loss).abs() <= 2 * miss * ez + 2.0 ** -19).all())
+    d, norms = 2.0 ** -22 * (lse.abs() + 1), Wd.norm(dim=1)
+    bound = d * (norms[at[:, 0]] + (z - lse[:, None]).exp() @ norms) + 2.0 ** -8 * (dz.abs() @ norms + dX.norm(dim=1))
+    assert bool(((grad.double() - dX).norm(dim=1) <= bound + 2 * miss * ez * norms.max()).all())
+
+
 @pytest.mark.parametrize("kind", ["mean", "spread", "tiny", "huge", "zeros", "signs"])
 def test_weights(k3, kind):
     """Incoming gradients as they come: a mean's 1/n, 40 orders of magnitude apart, all tiny or
