@@ -43,7 +43,7 @@
 // What bounds it: the tensor cores at the card's power limit. Alone, 2048 rows of 7168 over
 // 163,840 ids: the loss 3.12 ms (1.54 PFLOP/s, 0.91 of the measured burst rate), the gradient
 // 9.9 ms for the three products it runs (1.45), the tensor pipe 86-90% busy while the clock
-// falls to 1.34-1.46 GHz; back to back 14.8 ms together. A handful of rows is a weight
+// falls to 1.34-1.46 GHz; back to back 14.8-15.1 ms together. A handful of rows is a weight
 // stream: 9 rows 0.39 ms, 6.0 TB/s of W.
 // Units dealt out by a counter instead of in turn cost 2-3% (neighbouring SMs then no longer
 // read the same W tile together), pairs in the forward 3%.
