@@ -311,7 +311,7 @@ __device__ __forceinline__ int first_entry(const int *ids, int cnt, int v)
     int lo = 0, hi = cnt;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (__ldg(ids + mid) < v) lo = mid + 1;
+        if (ids[mid] < v) lo = mid + 1;
         else hi = mid;
     }
     return lo;
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
             __syncwarp();
             if (lane == 0) bar_arrive(s_addr(&b_took[slot]));
             const int row = words.y + rank * BM + q * 32 + lane;
-            if (words.x >= 0 && row < n_live) r = __ldg(a.rows + row);   // (of a dW unit it means nothing)
+            if (words.x >= 0 && row < n_live) r = a.rows[row];   // (of a dW unit it means nothing)
         };
         int4 words, words_next, r = make_int4(0, 0, 0, 0), r_next = r;
         for (take(words, r); words.x >= 0 && !failed; words = words_next, r = r_next) {
@@ -739,11 +739,8 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
 // mass = softmax(top / temp) over those. entropy = sum mass ln mass. The maximum carries a
 // NaN (fmaxf would drop it): such a row's masses, loss and gradient are NaN.
 constexpr int TEACHER_ROWS = 4, PER_LANE = MAXK / 32;
-__global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *__restrict__ s_ids, float *__restrict__ s_mass,
-                                                                    int *__restrict__ count,
-                                                                    float *__restrict__ entropy,
-                                                                    const int *__restrict__ ids,
-                                                                    const float *__restrict__ top, int T, int K,
+__global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *s_ids, float *s_mass, int *count, float *entropy,
+                                                                    const int *ids, const float *top, int T, int K,
                                                                     int vocab, float inv_temp)
 {
     __shared__ __align__(16) int sid_all[TEACHER_ROWS][MAXK];
@@ -918,11 +915,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
 #pragma unroll
                 for (int i = 0; i < PACK_COLS / 256; i++) {
                     const int c = c0 + (i * 32 + lane) * 8;
-                    if (c < c1) *reinterpret_cast<uint4 *>(o + c) = __ldg(reinterpret_cast<const uint4 *>(x + c));
+                    if (c < c1) *reinterpret_cast<uint4 *>(o + c) = *reinterpret_cast<const uint4 *>(x + c);
                 }
             } else {
 #pragma unroll 8
-                for (int c = c0 + lane; c < c1; c += 32) o[c] = __ldg(x + c);
+                for (int c = c0 + lane; c < c1; c += 32) o[c] = x[c];
             }
         }
         if (p < 0) {
@@ -941,11 +938,9 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
 }
 
 // 32 packed rows a block, 32 threads a row: the tile halves' statistics joined in double.
-__global__ void __launch_bounds__(1024) join_kernel(float *__restrict__ loss, float *__restrict__ lse,
-                                                    const float2 *__restrict__ part, int halves, int Tpad,
-                                                    const int4 *__restrict__ rows, const int *__restrict__ n_live,
-                                                    const float *__restrict__ zt, const float *__restrict__ mass,
-                                                    const float *__restrict__ entropy, int K, float c)
+__global__ void __launch_bounds__(1024) join_kernel(float *loss, float *lse, const float2 *part, int halves, int Tpad,
+                                                    const int4 *rows, const int *n_live, const float *zt,
+                                                    const float *mass, const float *entropy, int K, float c)
 {
     __shared__ float sm[32][33];
     __shared__ float ss[32][33];

@@ -3,6 +3,9 @@
 // before it touches any memory that another kernel may write or read: the wait returns when
 // every kernel before it has finished and its writes are visible. pdl_release() lets the next
 // kernel start its own set-up; it orders nothing.
+// Such a kernel is resident while the one before it still writes, so nothing that it reads is
+// constant over its lifetime: no read-only loads (ld.global.nc), neither by name nor through
+// `const ... __restrict__` parameters, which would also let the compiler move a load above the wait.
 #pragma once
 
 #include "common.cuh"

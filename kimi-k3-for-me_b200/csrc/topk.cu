@@ -179,8 +179,7 @@ __device__ __forceinline__ void write_out(const Shared &s, int *idx, float *val,
 
 // grid (segments, rows): the segment's K best, in order, to cand [rows][segments][K] (0 past its
 // candidates), or, of a row that is one segment, to idx and val
-__global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restrict__ cand, int *__restrict__ idx,
-                                                             float *__restrict__ val, const float *__restrict__ logits,
+__global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *cand, int *idx, float *val, const float *logits,
                                                              int vocab, int seg_len, int K)
 {
     __shared__ __align__(16) Shared s;
@@ -274,8 +273,7 @@ __global__ void __launch_bounds__(THREADS, 4) segment_kernel(uint64_t *__restric
 }
 
 // grid (rows): the K best of the segments' lists, in order
-__global__ void __launch_bounds__(THREADS) merge_kernel(int *__restrict__ idx, float *__restrict__ val,
-                                                        const uint64_t *__restrict__ cand, int nseg, int K)
+__global__ void __launch_bounds__(THREADS) merge_kernel(int *idx, float *val, const uint64_t *cand, int nseg, int K)
 {
     __shared__ __align__(16) Shared s;
     const int total = nseg * K;
