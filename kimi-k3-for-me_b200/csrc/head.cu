@@ -1297,6 +1297,13 @@ static bool head_ok(const uint16_t *X, int ldx, const uint16_t *W, int in, int v
     return X && W && ws && sizes_ok(T, in, vocab) && ldx >= in && aligned(W, 16) && aligned(X, 2) && aligned(ws, 256);
 }
 
+// 32-bit values on their boundaries (a NULL passes: what may not be absent is checked beside)
+template <typename... P>
+static bool words_ok(const P *...p)
+{
+    return (aligned(p, 4) && ...);
+}
+
 static bool grads_ok(const uint16_t *dX, int lddx, const uint16_t *dW, int in)
 {
     return (dX || dW) && (!dX || (lddx >= in && aligned(dX, 2))) && (!dW || aligned(dW, 16));
@@ -1305,7 +1312,7 @@ static bool grads_ok(const uint16_t *dX, int lddx, const uint16_t *dW, int in)
 static bool teacher_ok(const int *ids, const float *top, int K, float temp)
 {
     // (log2(e) / temp is what multiplies the logits)
-    return ids && top && K > 0 && K <= MAXK && temp > 0.0f && isfinite(temp) &&
+    return ids && top && words_ok(ids, top) && K > 0 && K <= MAXK && temp > 0.0f && isfinite(temp) &&
            isfinite((float)(1.4426950408889634 / (double)temp));
 }
 
@@ -1322,7 +1329,8 @@ extern "C" int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, in
                                   void *stream)
 {
     using namespace k3::head;
-    if (!loss || !lse || !label || !head_ok(X, ldx, W, in, vocab, T, workspace)) return K3GPU_EINVAL;
+    if (!loss || !lse || !label || !words_ok(loss, lse, label) || !head_ok(X, ldx, W, in, vocab, T, workspace))
+        return K3GPU_EINVAL;
     if (ws_bytes < workspace_bytes(T, in, vocab, 0)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, label, nullptr, nullptr, 0, 1.0f, k3::as_stream(stream)};
     return forward(loss, lse, c, workspace);
@@ -1333,7 +1341,8 @@ extern "C" int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, con
                                        int vocab, int T, void *workspace, size_t ws_bytes, void *stream)
 {
     using namespace k3::head;
-    if (!lse || !label || !head_ok(X, ldx, W, in, vocab, T, workspace) || !grads_ok(dX, lddx, dW, in))
+    if (!lse || !label || !words_ok(lse, label, g) || !head_ok(X, ldx, W, in, vocab, T, workspace) ||
+        !grads_ok(dX, lddx, dW, in))
         return K3GPU_EINVAL;
     if (ws_bytes < workspace_bytes(T, in, vocab, 0)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, label, nullptr, nullptr, 0, 1.0f, k3::as_stream(stream)};
@@ -1351,7 +1360,8 @@ extern "C" int k3gpu_lm_head_distill(float *loss, float *lse, const uint16_t *X,
                                      void *workspace, size_t ws_bytes, void *stream)
 {
     using namespace k3::head;
-    if (!loss || !lse || !teacher_ok(ids, top, K, temp) || !head_ok(X, ldx, W, in, vocab, T, workspace))
+    if (!loss || !lse || !words_ok(loss, lse) || !teacher_ok(ids, top, K, temp) ||
+        !head_ok(X, ldx, W, in, vocab, T, workspace))
         return K3GPU_EINVAL;
     if (ws_bytes < workspace_bytes(T, in, vocab, K)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, nullptr, ids, top, K, temp, k3::as_stream(stream)};
@@ -1364,7 +1374,7 @@ extern "C" int k3gpu_lm_head_distill_grad(uint16_t *dX, int lddx, uint16_t *dW, 
                                           void *workspace, size_t ws_bytes, void *stream)
 {
     using namespace k3::head;
-    if (!lse || !teacher_ok(ids, top, K, temp) || !head_ok(X, ldx, W, in, vocab, T, workspace) ||
+    if (!lse || !words_ok(lse, g) || !teacher_ok(ids, top, K, temp) || !head_ok(X, ldx, W, in, vocab, T, workspace) ||
         !grads_ok(dX, lddx, dW, in))
         return K3GPU_EINVAL;
     if (ws_bytes < workspace_bytes(T, in, vocab, K)) return K3GPU_ECAPACITY;

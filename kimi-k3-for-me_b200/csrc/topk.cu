@@ -331,7 +331,9 @@ extern "C" int k3gpu_topk_logits(int *idx, float *val, const float *logits, int 
 {
     using namespace k3::topk;
     if (!idx || !val || !logits || !workspace || rows <= 0 || vocab <= 0 || K <= 0 || K > MAXK) return K3GPU_EINVAL;
-    if (rows > 65535 || vocab > 1 << 30 || !k3::aligned(logits, 4) || !k3::aligned(workspace, 16)) return K3GPU_EINVAL;
+    if (rows > 65535 || vocab > 1 << 30 || !k3::aligned(logits, 4) || !k3::aligned(idx, 4) || !k3::aligned(val, 4) ||
+        !k3::aligned(workspace, 16))
+        return K3GPU_EINVAL;
     if (ws_bytes < k3gpu_topk_logits_workspace(rows, vocab, K)) return K3GPU_ECAPACITY;
     const int nseg = segments(rows, vocab);
     const int seg_len = k3::ceil_div(k3::ceil_div(vocab, nseg), 4) * 4;

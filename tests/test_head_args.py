@@ -106,3 +106,20 @@ def test_topk_refuses(m, kw):
 def test_topk_workspace_short(m):
     need = m.lib.k3gpu_topk_logits_workspace(9, 163840, 64)
     assert m.lib.k3gpu_topk_logits(P, P, P, 9, 163840, 64, P, need - 1, None) == m.K3GPU_ECAPACITY
+
+
+ODD = C.c_void_p((1 << 20) + 2)         # not on a 4-byte boundary
+
+
+@pytest.mark.parametrize("call,names", [(xent, ("loss", "lse", "label")), (xent_grad, ("lse", "label", "g")),
+                                        (distill, ("loss", "lse", "ids", "top")),
+                                        (distill_grad, ("lse", "ids", "top", "g"))])
+def test_misaligned_values_refused(m, call, names):
+    """32-bit inputs and outputs off their boundary: an error, not a fault of the kernels'."""
+    for name in names:
+        assert call(m, **{name: ODD}) == m.K3GPU_EINVAL, name
+
+
+def test_topk_misaligned_outputs_refused(m):
+    for idx, val in ((ODD, P), (P, ODD)):
+        assert m.lib.k3gpu_topk_logits(idx, val, P, 2, 10, 3, P, 1 << 20, None) == m.K3GPU_EINVAL
