@@ -587,9 +587,15 @@ def lm_head_argmax(X, W, ws=None, stream=None):
 
 
 # ------------------------------------------------------- fitting a draft head ------
+def _is_cuda_tensor(t):
+    return isinstance(t, torch.Tensor) and t.is_cuda
+
+
 def _on_device_of(fn):
     """Run a wrapper whose first argument is a CUDA tensor with that tensor's device current,
-    and, given a stream, with that stream current: what the call allocates then belongs to it."""
+    and, given a stream, with that stream current: what the call allocates then belongs to it, and
+    what it reads is recorded there, so that a temporary may be dropped before the kernels have run.
+    (That the stream waits for the inputs, and who reads the results for it, is the caller's.)"""
     @functools.wraps(fn)
     def call(x, *args, stream=None, **kw):
         if not x.is_cuda:
@@ -597,6 +603,9 @@ def _on_device_of(fn):
         if stream is not None:
             if stream.device != x.device:
                 raise K3Error(f"the stream is on {stream.device}, the tensors on {x.device}")
+            for t in (x, *args, *kw.values()):
+                if _is_cuda_tensor(t):
+                    t.record_stream(stream)
             with torch.cuda.stream(stream):
                 return fn(x, *args, **kw)
         if x.device.index == torch.cuda.current_device():
@@ -652,8 +661,11 @@ def _raw_stream(device):
 def topk_logits(logits, K, ws=None):
     """The K largest logits of each row of logits [rows][vocab]: (ids int32, values fp32)
     [rows][K], descending, equal values by ascending id, NaN never taken; a row that runs out
-    ends in id -1, -inf. The teacher entries of lm_head_distill. (This and the functions below also
-    take stream=, a torch.cuda.Stream to run on in place of the current one.)"""
+    ends in id -1, -inf. The teacher entries of lm_head_distill.
+
+    This and the functions below also take stream=, a torch.cuda.Stream to run on in place of the
+    current one. The caller lets that stream wait for what the inputs are made on, and waits for it
+    before the results, which belong to it, are used elsewhere; the inputs may be dropped at once."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
         raise K3Error(f"logits: expected contiguous fp32 [rows][vocab], got {logits.dtype} {tuple(logits.shape)}")
     (rows, vocab), dev = logits.shape, logits.device
