@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import inspect
 import os
 
 import torch
@@ -596,22 +597,30 @@ def _on_device_of(fn):
     and, given a stream, with that stream current: what the call allocates then belongs to it, and
     what it reads is recorded there, so that a temporary may be dropped before the kernels have run.
     (That the stream waits for the inputs, and who reads the results for it, is the caller's.)"""
+    sig = inspect.signature(fn)
+    first = next(iter(sig.parameters))
+
     @functools.wraps(fn)
-    def call(x, *args, stream=None, **kw):
+    def call(*args, stream=None, **kw):
+        x = args[0] if args else kw.get(first)
+        if x is None:
+            return fn(*args, **kw)                 # says which argument is missing
         if not x.is_cuda:
             raise K3Error("expected a CUDA tensor")
         if stream is not None:
             if stream.device != x.device:
                 raise K3Error(f"the stream is on {stream.device}, the tensors on {x.device}")
-            for t in (x, *args, *kw.values()):
+            for t in (*args, *kw.values()):
                 if _is_cuda_tensor(t):
                     t.record_stream(stream)
             with torch.cuda.stream(stream):
-                return fn(x, *args, **kw)
+                return fn(*args, **kw)
         if x.device.index == torch.cuda.current_device():
-            return fn(x, *args, **kw)
+            return fn(*args, **kw)
         with torch.cuda.device(x.device):
-            return fn(x, *args, **kw)
+            return fn(*args, **kw)
+    call.__signature__ = sig.replace(parameters=[
+        *sig.parameters.values(), inspect.Parameter("stream", inspect.Parameter.KEYWORD_ONLY, default=None)])
     return call
 
 

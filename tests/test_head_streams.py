@@ -80,6 +80,27 @@ def test_inputs_are_recorded_on_the_stream(k3, current, monkeypatch):
     assert x.seen == [s]
 
 
+def test_first_argument_by_name(k3, current):
+    """The first argument goes by its own name too, as help() shows it."""
+    call = k3._on_device_of(lambda X, y=0: (X, y))
+    x = Fake(1)
+    assert call(X=x, y=3) == (x, 3) and current == [x.device, None]
+    with pytest.raises(TypeError):
+        call(x=Fake())
+    with pytest.raises(TypeError):
+        call()
+    with pytest.raises(TypeError):
+        call(x, X=x)
+
+
+@pytest.mark.parametrize("name,first", [("topk_logits", "logits"), ("lm_head_xent", "X"), ("lm_head_xent_grad", "X"),
+                                        ("lm_head_distill", "X"), ("lm_head_distill_grad", "X")])
+def test_wrappers_take_their_first_argument_by_name(k3, name, first):
+    """Far enough to be told that a host tensor will not do."""
+    with pytest.raises(k3.K3Error, match="CUDA"):
+        getattr(k3, name)(**{first: torch.zeros(1)})
+
+
 # ------------------------------------------------------------------- on a device ------
 def inputs():
     gen = torch.Generator(device="cuda").manual_seed(1)
