@@ -632,6 +632,17 @@ def _arg(name, t, device, dtype, shape):
     return t.data_ptr()
 
 
+_MAXK = 128                     # entries of a row that the top-K gives and the distillation takes
+
+
+def _teacher_args(ids, top, device, T):
+    """(ids address, top address, K) of a row's teacher entries, checked."""
+    if ids.dim() != 2 or not 1 <= ids.shape[1] <= _MAXK:
+        raise K3Error(f"ids: expected [T][K] with K from 1 to {_MAXK}, got {tuple(ids.shape)}")
+    K = ids.shape[1]
+    return _arg("ids", ids, device, torch.int32, (T, K)), _arg("top", top, device, torch.float32, (T, K)), K
+
+
 _BF16_BITS = {torch.bfloat16, torch.int16, torch.uint16}
 
 
@@ -677,6 +688,8 @@ def topk_logits(logits, K, ws=None):
     before the results, which belong to it, are used elsewhere; the inputs may be dropped at once."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_contiguous():
         raise K3Error(f"logits: expected contiguous fp32 [rows][vocab], got {logits.dtype} {tuple(logits.shape)}")
+    if not 1 <= K <= _MAXK:
+        raise K3Error(f"K: expected 1 to {_MAXK}, got {K}")
     (rows, vocab), dev = logits.shape, logits.device
     idx = torch.empty(rows, K, dtype=torch.int32, device=dev)
     val = torch.empty(rows, K, dtype=torch.float32, device=dev)
@@ -738,8 +751,8 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
     negative id or a logit of -inf are empty; a row without entries has loss, lse and
     gradient 0."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
-    dev, K = X.device, ids.shape[-1]
-    ip, tp = _arg("ids", ids, dev, torch.int32, (T, K)), _arg("top", top, dev, torch.float32, (T, K))
+    dev = X.device
+    ip, tp, K = _teacher_args(ids, top, dev, T)
     loss = torch.empty(T, dtype=torch.float32, device=dev)
     lse = torch.empty(T, dtype=torch.float32, device=dev)
     if T == 0:
@@ -754,8 +767,8 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
 def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, need_dw=True, ws=None):
     """The gradient of lm_head_distill (arguments and results as lm_head_xent_grad)."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
-    dev, K = X.device, ids.shape[-1]
-    ip, tp = _arg("ids", ids, dev, torch.int32, (T, K)), _arg("top", top, dev, torch.float32, (T, K))
+    dev = X.device
+    ip, tp, K = _teacher_args(ids, top, dev, T)
     ls = _arg("lse", lse, dev, torch.float32, (T,))
     gp = _arg("g", g, dev, torch.float32, (T,)) if g is not None else None
     dX, dx, dW, dw = _grads(X, W, need_dx, need_dw)

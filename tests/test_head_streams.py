@@ -101,6 +101,43 @@ def test_wrappers_take_their_first_argument_by_name(k3, name, first):
         getattr(k3, name)(**{first: torch.zeros(1)})
 
 
+class FakeTensor(Fake):
+    """As far as a wrapper's checks look before anything is allocated."""
+
+    def __init__(self, dtype, *shape):
+        super().__init__()
+        self.dtype, self.shape = dtype, torch.Size(shape)
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return True
+
+    def stride(self):
+        return torch.empty(self.shape, device="meta").stride()
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+@pytest.mark.parametrize("K", [-1, 0, 129])
+def test_topk_refuses_k_before_it_allocates(k3, current, K, rows):
+    with pytest.raises(k3.K3Error, match="K"):
+        k3.topk_logits(FakeTensor(torch.float32, rows, 100), K)
+
+
+@pytest.mark.parametrize("shape", [(), (8,), (8, 2, 2), (8, 0), (8, 129)])
+def test_distill_refuses_entries_of_another_shape(k3, current, shape):
+    X, W = FakeTensor(torch.bfloat16, 8, 64), FakeTensor(torch.bfloat16, 100, 64)
+    ids, top, lse = FakeTensor(torch.int32, *shape), FakeTensor(torch.float32, *shape), FakeTensor(torch.float32, 8)
+    with pytest.raises(k3.K3Error, match="ids"):
+        k3.lm_head_distill(X, W, ids, top)
+    with pytest.raises(k3.K3Error, match="ids"):
+        k3.lm_head_distill_grad(X, W, ids, top, lse)
+
+
 # ------------------------------------------------------------------- on a device ------
 def inputs():
     gen = torch.Generator(device="cuda").manual_seed(1)
