@@ -411,15 +411,24 @@ int k3gpu_topk_logits(int *idx, float *val, const float *logits, int rows, int v
  * [T][vocab] logits are never written). X [T][in] bf16 bits, row stride ldx elements (any
  * ldx >= in; rows on 16-byte boundaries are best), W [vocab][in] bf16 bits,
  * 16-byte aligned; z = X W^T with exact products and fp32 sums.
- * Limits: in % 8 == 0, in <= 65536, vocab <= 2^24, T <= 2^20; the workspace is 256-byte
- * aligned, the same for a loss and its gradient. The reference has no training code; these
- * have no counterpart there.
+ * Limits: in % 8 == 0, in <= 65536, vocab <= 2^24, T <= 2^20. The reference has no training
+ * code; these have no counterpart there.
+ *
+ * The workspace is 256-byte aligned. A loss alone needs *_loss_workspace() bytes: a copy of the
+ * hidden states (rows padded to 256) and, a row, 16 bytes for every 256 ids (a sixty-fourth of
+ * fp32 logits). *_workspace() bytes serve a loss and its gradient, which needs that copy, dz in bf16
+ * and dX's sums in fp32. dz (rows padded to 64) is whole where 256-padded rows of it take up to 128
+ * MB; for few rows it and the sums are larger than their logits. Else it is two pieces of up to 128
+ * MB (of 2048 ids above 32,768 rows). The sums (rows padded to 32) are split up to 32 times, within
+ * 256 MB, or one dX in fp32 where that is larger. Of 7168 columns over 163,840 ids: 9 rows 6.5
+ * MB for the loss and 47 MB for both, 2048 rows 51 and 416 MB.
  *
  * Softmax cross entropy: lse[t] = ln sum_v e^z[t][v], loss[t] = lse[t] - z[t][label[t]], fp32
  * [T]. A negative label is a row without a target: its loss, lse and gradient are 0, and
  * nothing of its hidden state is read. A label >= vocab is treated so and flagged (device
  * status bit 1). */
 size_t k3gpu_lm_head_xent_workspace(int T, int in, int vocab);
+size_t k3gpu_lm_head_xent_loss_workspace(int T, int in, int vocab);
 int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, int ldx, const uint16_t *W,
                        const int *label, int in, int vocab, int T, void *workspace,
                        size_t ws_bytes, void *stream);
@@ -427,9 +436,8 @@ int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, int ldx, cons
  *   dz[t][v] = g[t] (e^(z[t][v] - lse[t]) - [v == label[t]]),  dX = dz W,  dW = dz^T X
  * with g [T] the loss's incoming gradient (NULL: 1). dX [T][in] (row stride lddx) and dW
  * [vocab][in] (16-byte aligned) are bf16 bits, written whole, not added to; either may be
- * NULL (a frozen head needs no dW). dz is rounded to bf16 once; the sums are fp32. The
- * vocabulary is taken in pieces: of the size of the logits the workspace holds a sixty-fourth
- * (the loss's running statistics). Neither output may overlap an input. */
+ * NULL (a frozen head needs no dW). dz is rounded to bf16 once; the sums are fp32. Neither
+ * output may overlap an input. */
 int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, const float *g,
                             const float *lse, const uint16_t *X, int ldx, const uint16_t *W,
                             const int *label, int in, int vocab, int T, void *workspace,
@@ -443,6 +451,7 @@ int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, const float *g
  * gradient 0 and its hidden state is not read. A NaN or +inf teacher logit makes its row's
  * loss NaN. 1 <= K <= 128. */
 size_t k3gpu_lm_head_distill_workspace(int T, int in, int vocab, int K);
+size_t k3gpu_lm_head_distill_loss_workspace(int T, int in, int vocab, int K);
 int k3gpu_lm_head_distill(float *loss, float *lse, const uint16_t *X, int ldx, const uint16_t *W,
                           const int *ids, const float *top, int K, float temp, int in, int vocab,
                           int T, void *workspace, size_t ws_bytes, void *stream);

@@ -210,9 +210,11 @@ _SIGS = {
     "k3gpu_topk_logits_workspace": ([I, I, I], SZ),
     "k3gpu_topk_logits": ([VP, VP, VP, I, I, I, VP, SZ, VP], I),
     "k3gpu_lm_head_xent_workspace": ([I, I, I], SZ),
+    "k3gpu_lm_head_xent_loss_workspace": ([I, I, I], SZ),
     "k3gpu_lm_head_xent": ([VP, VP, VP, I, VP, VP, I, I, I, VP, SZ, VP], I),
     "k3gpu_lm_head_xent_grad": ([VP, I, VP, VP, VP, VP, I, VP, VP, I, I, I, VP, SZ, VP], I),
     "k3gpu_lm_head_distill_workspace": ([I, I, I, I], SZ),
+    "k3gpu_lm_head_distill_loss_workspace": ([I, I, I, I], SZ),
     "k3gpu_lm_head_distill": ([VP, VP, VP, I, VP, VP, VP, I, F, I, I, I, VP, SZ, VP], I),
     "k3gpu_lm_head_distill_grad": ([VP, I, VP, VP, VP, VP, I, VP, VP, VP, I, F, I, I, I, VP, SZ, VP], I),
     "k3gpu_attn_res": ([VP, VP, VP, VP, VP, I, I, I, F, VP], I),
@@ -713,7 +715,7 @@ def lm_head_xent(X, W, label, ws=None):
     lse = torch.empty(T, dtype=torch.float32, device=dev)
     if T == 0:
         return loss, lse
-    ws = _scratch(ws, lib.k3gpu_lm_head_xent_workspace(T, n, vocab), dev)
+    ws = _scratch(ws, lib.k3gpu_lm_head_xent_loss_workspace(T, n, vocab), dev)
     check(lib.k3gpu_lm_head_xent(loss.data_ptr(), lse.data_ptr(), xp, ldx, w, lab, n, vocab, T, ws.data_ptr(),
                                  ws.numel(), _raw_stream(dev)), "k3gpu_lm_head_xent")
     return loss, lse
@@ -757,7 +759,7 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
     lse = torch.empty(T, dtype=torch.float32, device=dev)
     if T == 0:
         return loss, lse
-    ws = _scratch(ws, lib.k3gpu_lm_head_distill_workspace(T, n, vocab, K), dev)
+    ws = _scratch(ws, lib.k3gpu_lm_head_distill_loss_workspace(T, n, vocab, K), dev)
     check(lib.k3gpu_lm_head_distill(loss.data_ptr(), lse.data_ptr(), xp, ldx, w, ip, tp, K, float(temp), n, vocab, T,
                                     ws.data_ptr(), ws.numel(), _raw_stream(dev)), "k3gpu_lm_head_distill")
     return loss, lse

@@ -83,7 +83,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 enum Mode { LOSS, GRAD };
 enum Kind { Z, DX, DW };                   // what a unit of work forms
 
-// A vocabulary piece of the backward: ids v0 .. v0 + vc - 1, their dz [Tpad][piece].
+// A vocabulary piece of the backward: ids v0 .. v0 + vc - 1, their dz [dz_rows][piece].
 struct Piece {
     int v0, vc;
     __nv_bfloat16 *dz;
@@ -110,8 +110,10 @@ struct Args {
     float inv_temp;
     Piece d;                    // vc = 0: no dX and dW units in this launch
     int want_dx, want_dw, first, last;
+    int dz_rows;                // rows that dz has a place for: T rounded up to a K step of dW
     int splits, split_steps;    // dX: K splits, 64-K steps of each
-    float4 *acc;                // dX before its last sum: by split, 128 x 256 tile, warp, 4 columns, lane
+    int acc_groups;             // 32-row groups of acc, to the end of T
+    float4 *acc;                // dX before its last sum: by split, 32 rows x 128 columns, 4 columns, lane
     __nv_bfloat16 *dX;
     int lddx, vec_dx;
     int z_before_dw;            // the longer units come first
@@ -393,6 +395,7 @@ __device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *ou
         for (int j = 0; j < HALF; j++) z[j] = 0.0f;
         gt = 0.0f;
     }
+    if (row0 >= a.dz_rows) return;         // (a multiple of 64: a warp's 32 rows lie on one side of it)
 #pragma unroll
     for (int c0 = 0; c0 < HALF; c0 += 64)
         store64(buf, out, col0 + c0, row0, false, lane, [&](int j) {
@@ -404,11 +407,11 @@ __device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *ou
 
 // dz was formed without these: exactly common factors add no rounding of their own to it
 __device__ __forceinline__ float out_scale(const Args &a) { return (a.g_scale ? *a.g_scale : 1.0f) * a.inv_temp; }
-// where a warp's part of a dX tile lies in acc (float4s; its lanes follow)
-__device__ __forceinline__ size_t acc_at(const Args &a, int split, int row0, int col0, int w)
+// where a warp's 32 rows x 128 columns of a dX tile lie in acc (float4s; its lanes follow)
+__device__ __forceinline__ size_t acc_at(const Args &a, int split, int row0, int col0)
 {
-    const size_t tile = ((size_t)split * (a.Tpad / BM) + row0 / BM) * ((a.in + BN - 1) / BN) + col0 / BN;
-    return (tile * 8 + w) * (HALF / 4) * 32;
+    const size_t groups = (size_t)split * a.acc_groups + row0 / 32;
+    return (groups * ((a.in + BN - 1) / BN * 2) + col0 / HALF) * (HALF / 4) * 32;
 }
 __device__ __forceinline__ void put8(__nv_bfloat16 *out, const float4 &f0, const float4 &f1, float k, bool vec)
 {
@@ -657,7 +660,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 const bool live = row < n_live;
                 const float scale = out_scale(a);
                 const bool sum = a.splits > 1 || !a.last, add = !a.first;
-                float4 *acc = a.acc + acc_at(a, t.split, t.m0 + rank * BM, t.n0, warp - 2) + lane;
+                float4 *acc = a.acc + acc_at(a, t.split, row0, col0) + lane;
                 __nv_bfloat16 *out = live ? a.dX + (size_t)r.x * a.lddx : nullptr;
                 take(words_next, r_next);
                 if (t.steps > 0 && !finished()) { failed = true; break; }
@@ -713,18 +716,19 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
 }
 
 // dX = the splits' sums in order, as bf16. Block (tile, p): columns 8 p .. and 128 + 8 p .. of a
-// 128 x 256 tile, a warp per epilogue warp's part.
+// 128 x 256 tile, a warp for 32 rows of each half.
 __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
 {
     const int cols = (a.in + BN - 1) / BN, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row0 = (int)(blockIdx.x / cols) * BM, n0 = (int)(blockIdx.x % cols) * BN;
-    const int row = row0 + ((w + 2) & 3) * 32 + lane, col = n0 + (w >> 2) * HALF + (int)blockIdx.y * 8;
+    const int group = row0 + (w & 3) * 32, row = group + lane, half = n0 + (w >> 2) * HALF;
+    const int col = half + (int)blockIdx.y * 8;
     pdl_wait();
     pdl_release();
     if (row >= *a.n_live || col >= a.in) return;
     float4 f0 = make_float4(0, 0, 0, 0), f1 = f0;
-    const float4 *p = a.acc + acc_at(a, 0, row0, n0, w) + (int)blockIdx.y * 64 + lane;
-    const size_t step = acc_at(a, 1, 0, 0, 0);
+    const float4 *p = a.acc + acc_at(a, 0, group, half) + (int)blockIdx.y * 64 + lane;
+    const size_t step = acc_at(a, 1, 0, 0);
 #pragma unroll 4
     for (int s = 0; s < a.splits; s++, p += step) {
         const float4 p0 = p[0], p1 = p[32];
@@ -1038,13 +1042,19 @@ static int map2d(CUtensorMap *m, const void *base, long long cols, long long ld,
 
 constexpr long long MAX_T = 1 << 20, MAX_VOCAB = 1 << 24, MAX_IN = 1 << 16;
 
+constexpr size_t MAX_SUMS = 256 << 20;
+// workspaces come in whole 256 KB: batches of about one size share one, and the smallest have one size
+// for both directions
+constexpr size_t GRAIN = 256 << 10;
+
 static size_t a256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct Plan {
     int cg;                            // CTAs that share a unit of the backward
     int Tpad, tiles, piece, pieces;    // vocabulary tiles; ids per piece of the backward; pieces
+    int dz_rows, acc_groups;           // rows of dz, 32-row groups of dX's sums
     int splits, split_steps;           // of dX's K (a piece)
-    size_t dz_bytes;                   // of one piece
+    size_t dz_bytes, acc_bytes;        // of one piece; of dX's sums in fp32
 };
 
 // The steps of the busiest worker when units of three kinds are dealt out in turn: each kind
@@ -1077,16 +1087,20 @@ static Plan plan(int T, int in, int vocab)
     const long long tiles = std::max<long long>(8, (128LL << 20) / ((long long)p.Tpad * 2 * BN));
     p.piece = (int)std::min<long long>(tiles, p.tiles) * BN;
     p.pieces = ceil_div(vocab, p.piece);
-    p.dz_bytes = (size_t)p.Tpad * p.piece * 2;
+    p.dz_rows = ceil_div(T, KB) * KB;
+    p.dz_bytes = (size_t)p.dz_rows * p.piece * 2;
     // dX has few tiles with long sums over the ids: split them where that shortens the busiest
     // worker of the launches (148 SMs), each unit's fp32 sums costing about 16 steps to write
-    // and read back
+    // and read back; the sums of all splits take 256 MB at most (a limit that only hidden states
+    // wider than 19,000 reach)
     const int rows = ceil_div(T, BM * p.cg), cols = ceil_div(in, BN), steps = p.piece / KB, workers = 148 / p.cg;
     const long long n_w = (long long)ceil_div(p.piece, BM * p.cg) * cols, n_z = (long long)rows * (p.piece / BN);
+    p.acc_groups = ceil_div(T, 32);
+    const size_t sums = (size_t)p.acc_groups * 32 * cols * BN * 4;
     double best = 0.0;
     p.splits = 1;
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-        if (s > 1 && steps / s < 4) break;
+        if (s > 1 && (steps / s < 4 || s * sums > MAX_SUMS)) break;
         const int len = ceil_div(steps, s);
         const double cost[3] = {len + (s > 1 || p.pieces > 1 ? 16.0 : 4.0), ceil_div(T, KB) + 4.0,
                                 ceil_div(in, KB) + 4.0};
@@ -1099,6 +1113,7 @@ static Plan plan(int T, int in, int vocab)
     }
     p.split_steps = ceil_div(steps, p.splits);
     p.splits = ceil_div(steps, p.split_steps);
+    p.acc_bytes = p.pieces > 1 || p.splits > 1 ? p.splits * sums : 0;
     return p;
 }
 
@@ -1137,10 +1152,10 @@ static size_t layout(Ws *w, char *base, const Plan &p, int T, int in, int K, boo
     } else {
         x.dz[0] = (__nv_bfloat16 *)take(p.dz_bytes);
         x.dz[1] = p.pieces > 1 ? (__nv_bfloat16 *)take(p.dz_bytes) : x.dz[0];
-        if (p.pieces > 1 || p.splits > 1) x.acc = (float4 *)take((size_t)p.splits * p.Tpad * ceil_div(in, BN) * BN * 4);
+        if (p.acc_bytes) x.acc = (float4 *)take(p.acc_bytes);
     }
     if (w) *w = x;
-    return o;
+    return (o + GRAIN - 1) / GRAIN * GRAIN;
 }
 
 static bool sizes_ok(int T, int in, int vocab)
@@ -1261,6 +1276,7 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     if ((st = set_up(&a, &maps, c, p, w, k, p.cg, true))) return st;
     a.g_scale = g ? w.g_scale : nullptr;
     a.acc = w.acc;
+    a.dz_rows = p.dz_rows; a.acc_groups = p.acc_groups;
     a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);
     a.want_dx = dX != nullptr; a.want_dw = dW != nullptr;
@@ -1272,10 +1288,10 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
         a.first = i == 1; a.last = i == p.pieces;
         const int v0 = i * p.piece;
         a.z = i < p.pieces ? Piece{v0, std::min(p.piece, c.vocab - v0), w.dz[i & 1]} : Piece{};
-        if (i < p.pieces && (st = map2d(&maps.z_out, a.z.dz, p.piece, p.piece, p.Tpad, 32))) return st;
+        if (i < p.pieces && (st = map2d(&maps.z_out, a.z.dz, p.piece, p.piece, p.dz_rows, 32))) return st;
         if (i > 0) {
-            if ((st = map2d(&maps.dz_k, a.d.dz, a.d.vc, p.piece, p.Tpad, BM))) return st;
-            if ((st = map2d(&maps.dz_mn, a.d.dz, a.d.vc, p.piece, p.Tpad, 64))) return st;
+            if ((st = map2d(&maps.dz_k, a.d.dz, a.d.vc, p.piece, p.dz_rows, BM))) return st;
+            if ((st = map2d(&maps.dz_mn, a.d.dz, a.d.vc, p.piece, p.dz_rows, 64))) return st;
         }
         st = p.cg == 1 ? launch_head<GRAD, 1>(maps, a, sms, c.s) : launch_head<GRAD, 2>(maps, a, sms, c.s);
         if (st) return st;
@@ -1286,10 +1302,14 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     return K3GPU_OK;
 }
 
-static size_t workspace_bytes(int T, int in, int vocab, int K)
+// what one direction needs (K = 0: cross entropy)
+static size_t workspace_bytes(int T, int in, int vocab, int K, bool grad)
 {
-    const Plan p = plan(T, in, vocab);
-    return std::max(layout(nullptr, nullptr, p, T, in, K, false), layout(nullptr, nullptr, p, T, in, K, true));
+    return layout(nullptr, nullptr, plan(T, in, vocab), T, in, K, grad);
+}
+static size_t workspace_both(int T, int in, int vocab, int K)
+{
+    return std::max(workspace_bytes(T, in, vocab, K, false), workspace_bytes(T, in, vocab, K, true));
 }
 
 static bool head_ok(const uint16_t *X, int ldx, const uint16_t *W, int in, int vocab, int T, const void *ws)
@@ -1321,7 +1341,12 @@ static bool teacher_ok(const int *ids, const float *top, int K, float temp)
 
 extern "C" size_t k3gpu_lm_head_xent_workspace(int T, int in, int vocab)
 {
-    return k3::head::sizes_ok(T, in, vocab) ? k3::head::workspace_bytes(T, in, vocab, 0) : 0;
+    return k3::head::sizes_ok(T, in, vocab) ? k3::head::workspace_both(T, in, vocab, 0) : 0;
+}
+
+extern "C" size_t k3gpu_lm_head_xent_loss_workspace(int T, int in, int vocab)
+{
+    return k3::head::sizes_ok(T, in, vocab) ? k3::head::workspace_bytes(T, in, vocab, 0, false) : 0;
 }
 
 extern "C" int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, int ldx, const uint16_t *W,
@@ -1331,7 +1356,7 @@ extern "C" int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, in
     using namespace k3::head;
     if (!loss || !lse || !label || !words_ok(loss, lse, label) || !head_ok(X, ldx, W, in, vocab, T, workspace))
         return K3GPU_EINVAL;
-    if (ws_bytes < workspace_bytes(T, in, vocab, 0)) return K3GPU_ECAPACITY;
+    if (ws_bytes < workspace_bytes(T, in, vocab, 0, false)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, label, nullptr, nullptr, 0, 1.0f, k3::as_stream(stream)};
     return forward(loss, lse, c, workspace);
 }
@@ -1344,7 +1369,7 @@ extern "C" int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, con
     if (!lse || !label || !words_ok(lse, label, g) || !head_ok(X, ldx, W, in, vocab, T, workspace) ||
         !grads_ok(dX, lddx, dW, in))
         return K3GPU_EINVAL;
-    if (ws_bytes < workspace_bytes(T, in, vocab, 0)) return K3GPU_ECAPACITY;
+    if (ws_bytes < workspace_bytes(T, in, vocab, 0, true)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, label, nullptr, nullptr, 0, 1.0f, k3::as_stream(stream)};
     return backward(dX, lddx, dW, g, lse, c, workspace);
 }
@@ -1352,7 +1377,13 @@ extern "C" int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, con
 extern "C" size_t k3gpu_lm_head_distill_workspace(int T, int in, int vocab, int K)
 {
     using namespace k3::head;
-    return sizes_ok(T, in, vocab) && K > 0 && K <= MAXK ? workspace_bytes(T, in, vocab, K) : 0;
+    return sizes_ok(T, in, vocab) && K > 0 && K <= MAXK ? workspace_both(T, in, vocab, K) : 0;
+}
+
+extern "C" size_t k3gpu_lm_head_distill_loss_workspace(int T, int in, int vocab, int K)
+{
+    using namespace k3::head;
+    return sizes_ok(T, in, vocab) && K > 0 && K <= MAXK ? workspace_bytes(T, in, vocab, K, false) : 0;
 }
 
 extern "C" int k3gpu_lm_head_distill(float *loss, float *lse, const uint16_t *X, int ldx, const uint16_t *W,
@@ -1363,7 +1394,7 @@ extern "C" int k3gpu_lm_head_distill(float *loss, float *lse, const uint16_t *X,
     if (!loss || !lse || !words_ok(loss, lse) || !teacher_ok(ids, top, K, temp) ||
         !head_ok(X, ldx, W, in, vocab, T, workspace))
         return K3GPU_EINVAL;
-    if (ws_bytes < workspace_bytes(T, in, vocab, K)) return K3GPU_ECAPACITY;
+    if (ws_bytes < workspace_bytes(T, in, vocab, K, false)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, nullptr, ids, top, K, temp, k3::as_stream(stream)};
     return forward(loss, lse, c, workspace);
 }
@@ -1377,7 +1408,7 @@ extern "C" int k3gpu_lm_head_distill_grad(uint16_t *dX, int lddx, uint16_t *dW, 
     if (!lse || !words_ok(lse, g) || !teacher_ok(ids, top, K, temp) || !head_ok(X, ldx, W, in, vocab, T, workspace) ||
         !grads_ok(dX, lddx, dW, in))
         return K3GPU_EINVAL;
-    if (ws_bytes < workspace_bytes(T, in, vocab, K)) return K3GPU_ECAPACITY;
+    if (ws_bytes < workspace_bytes(T, in, vocab, K, true)) return K3GPU_ECAPACITY;
     const Call c{X, W, ldx, in, vocab, T, nullptr, ids, top, K, temp, k3::as_stream(stream)};
     return backward(dX, lddx, dW, g, lse, c, workspace);
 }
