@@ -707,7 +707,11 @@ def topk_logits(logits, K, ws=None):
 def lm_head_xent(X, W, label, ws=None):
     """Softmax cross entropy of the lm_head product X [T][in] . W^T (bf16, the logits never
     written) against label int32 [T]: (loss, lse) fp32 [T]. A negative label is a row without a
-    target: loss, lse and gradient 0."""
+    target: loss, lse and gradient 0.
+
+    This and the functions below are outside autograd: an X or W that requires grad is taken, and
+    what comes back carries no graph. Go on from the _grad function's results: X.backward(dX) takes dX
+    into the model that made X, dW is W's gradient."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
     dev = X.device
     lab = _arg("label", label, dev, torch.int32, (T,))
@@ -733,7 +737,8 @@ def _grads(X, W, need_dx, need_dw):
 @_on_device_of
 def lm_head_xent_grad(X, W, label, lse, g=None, need_dx=True, need_dw=True, ws=None):
     """The gradient of lm_head_xent from its lse and the loss's incoming gradient g fp32 [T]
-    (None: 1): (dX [T][in], dW [vocab][in]) bf16, None where not needed (a frozen head)."""
+    (None: 1): (dX [T][in], dW [vocab][in]) bf16, None where not needed (a frozen head). Outside
+    autograd, as lm_head_xent."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
     dev = X.device
     lab, ls = _arg("label", label, dev, torch.int32, (T,)), _arg("lse", lse, dev, torch.float32, (T,))
@@ -751,7 +756,7 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
     """KL of the teacher's top logits (ids int32, top fp32 [T][K], e.g. topk_logits of its
     sweep) from the head's softmax, both at temperature temp: (loss, lse) fp32 [T]. Entries with a
     negative id or a logit of -inf are empty; a row without entries has loss, lse and
-    gradient 0."""
+    gradient 0. Outside autograd, as lm_head_xent."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
     dev = X.device
     ip, tp, K = _teacher_args(ids, top, dev, T)
@@ -767,7 +772,8 @@ def lm_head_distill(X, W, ids, top, temp=1.0, ws=None):
 
 @_on_device_of
 def lm_head_distill_grad(X, W, ids, top, lse, temp=1.0, g=None, need_dx=True, need_dw=True, ws=None):
-    """The gradient of lm_head_distill (arguments and results as lm_head_xent_grad)."""
+    """The gradient of lm_head_distill (arguments and results as lm_head_xent_grad). Outside autograd,
+    as lm_head_xent."""
     xp, ldx, w, n, vocab, T = _head_args(X, W)
     dev = X.device
     ip, tp, K = _teacher_args(ids, top, dev, T)

@@ -1,5 +1,6 @@
 """The draft-head wrappers on a stream or device that is not the current one: the device that they
-make current, the names of their arguments, and how long what a call reads stays alive."""
+make current, the names of their arguments, how long what a call reads stays alive, and how a model
+in torch goes on from their gradients."""
 import contextlib
 import os
 import sys
@@ -138,6 +139,11 @@ def test_distill_refuses_entries_of_another_shape(k3, current, shape):
         k3.lm_head_distill_grad(X, W, ids, top, lse)
 
 
+@pytest.mark.parametrize("name", ["lm_head_xent", "lm_head_xent_grad", "lm_head_distill", "lm_head_distill_grad"])
+def test_documented_as_outside_autograd(k3, name):
+    assert "utside autograd" in " ".join(getattr(k3, name).__doc__.split())
+
+
 # ------------------------------------------------------------------- on a device ------
 def inputs():
     gen = torch.Generator(device="cuda").manual_seed(1)
@@ -187,3 +193,24 @@ def test_a_temporary_outlives_its_call(k3, which):
     side.synchronize()
     for a, b in zip(got[0], want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_model_in_torch_goes_on_from_the_gradients(k3):
+    """Parameters that require grad: the loss carries no graph, X.backward(dX) takes the gradient into
+    the model that made X, dW is the head's."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn((40, 64), generator=gen, device="cuda")
+    trunk = torch.nn.Parameter(torch.randn((128, 64), generator=gen, device="cuda") / 8)
+    head = torch.nn.Parameter((torch.randn((500, 128), generator=gen, device="cuda") / 11).bfloat16())
+    label = torch.randint(-1, 500, (40,), generator=gen, device="cuda").int()
+    X = (x @ trunk.T).bfloat16()
+    loss, lse = k3.lm_head_xent(X, head, label)
+    dX, head.grad = k3.lm_head_xent_grad(X, head, label, lse)
+    assert not loss.requires_grad and not dX.requires_grad
+    X.backward(dX)
+    assert torch.equal(trunk.grad, torch.autograd.grad((x @ trunk.T).bfloat16(), trunk, dX)[0])
+    assert float(trunk.grad.norm()) > 0 and head.grad.shape == head.shape
+    # the same as from tensors that require none
+    d, w = k3.lm_head_xent_grad(X.detach(), head.detach(), label, lse)
+    assert torch.equal(d, dX) and torch.equal(w, head.grad)
