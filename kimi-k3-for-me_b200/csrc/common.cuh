@@ -49,6 +49,10 @@ inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s
 
 inline bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// SMs of a B200: what a plan that a workspace query must agree with is made for (a query needs no
+// device). Launches ask the device.
+constexpr int PLAN_SMS = 148;
+
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // 1 / (1 + exp(-v)) in float with a correctly rounded exp: the double exp of CUDA's

@@ -1077,8 +1077,8 @@ static Plan plan(int T, int in, int vocab)
 {
     Plan p;
     // Pairs take 7% less time a row where both halves of their 256-row tiles are full (2048 x
-    // 7168 over 163,840 ids: 15.4 against 16.4 ms for loss and gradient); 576 rows, 2.5 of
-    // their tiles, take 18% more.
+    // 7168 over 163,840 ids: 15.4 against 16.4 ms for loss and gradient); 576 rows, 2.25
+    // of their tiles, take 18% more.
     p.cg = 100LL * ceil_div(T, 2 * BM) * 2 < 107LL * ceil_div(T, BM) ? 2 : 1;
     p.Tpad = ceil_div(T, ROW_PAD) * ROW_PAD;
     p.tiles = ceil_div(vocab, BN);
@@ -1090,10 +1090,11 @@ static Plan plan(int T, int in, int vocab)
     p.dz_rows = ceil_div(T, KB) * KB;
     p.dz_bytes = (size_t)p.dz_rows * p.piece * 2;
     // dX has few tiles with long sums over the ids: split them where that shortens the busiest
-    // worker of the launches (148 SMs), each unit's fp32 sums costing about 16 steps to write
+    // worker of the launches, each unit's fp32 sums costing about 16 steps to write
     // and read back; the sums of all splits take 256 MB at most (a limit that only hidden states
     // wider than 19,000 reach)
-    const int rows = ceil_div(T, BM * p.cg), cols = ceil_div(in, BN), steps = p.piece / KB, workers = 148 / p.cg;
+    const int rows = ceil_div(T, BM * p.cg), cols = ceil_div(in, BN), steps = p.piece / KB;
+    const int workers = PLAN_SMS / p.cg;
     const long long n_w = (long long)ceil_div(p.piece, BM * p.cg) * cols, n_z = (long long)rows * (p.piece / BN);
     p.acc_groups = ceil_div(T, 32);
     const size_t sums = (size_t)p.acc_groups * 32 * cols * BN * 4;

@@ -308,9 +308,9 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(int *idx, float *val, co
 
 static int segments(int rows, int vocab)
 {
-    // at most four blocks an SM (of 148), one wave, no segment shorter than a round: 576 rows in
+    // at most four blocks an SM, one wave, no more segments than the row has rounds: 576 rows in
     // one segment each take 63 us (in two, before the loads ran ahead, 76 against 69)
-    const int want = 4 * 148 / rows, most = ceil_div(vocab, ROUND);
+    const int want = 4 * PLAN_SMS / rows, most = ceil_div(vocab, ROUND);
     return std::max(1, std::min(std::min(want, most), MAX_SEG));
 }
 
