@@ -25,6 +25,13 @@
 // it (1/temp, the largest weight's mantissa; the outputs get them in fp32) and is rounded to bf16
 // once: at most 2^-8 of an element, as much as the outputs' own rounding, independent
 // between elements. All sums are fp32.
+// Few elements that matter do not average that rounding out (4 rows of 2 entries: dX off by
+// 0.0025, by 0.0016 with an exact dz). Up to 32 rows a tile has room for as many again: there the
+// rest of each rounding, as bf16, is a second set of rows, against W for dX (whose last sum joins
+// the two) and against a copy of X for dW; rows and rests together are one K step of it, the
+// products no more tiles than without. Loss and gradient of 4 rows of 1024 over 32,000 ids take 84
+// us against 80, of 32 rows of 7168 over 163,840 1.81 ms against 1.77. (Up to 64 rows it was two
+// K steps: 127 against 101 us at 64 rows of 1024, which are off by 0.0019 to 0.0024 without.)
 //
 // One persistent CTA per SM takes every n-th unit of work (10 warps):
 //   warp 0     TMA, a ring of 64-K stages: A 128 rows (16 KB), B 256 rows (32 KB)
@@ -80,7 +87,7 @@ constexpr int ROW_PAD = 2 * BM;            // packed rows end on a pair's tile
 constexpr int PACK_BLOCKS = 512, PACK_ROWS = 2048, PACK_COLS = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
-enum Mode { LOSS, GRAD };
+enum Mode { LOSS, GRAD, GRAD_RESTS };      // GRAD_RESTS: dz in two parts (Args::rest)
 enum Kind { Z, DX, DW };                   // what a unit of work forms
 
 // A vocabulary piece of the backward: ids v0 .. v0 + vc - 1, their dz [dz_rows][piece].
@@ -111,6 +118,7 @@ struct Args {
     Piece d;                    // vc = 0: no dX and dW units in this launch
     int want_dx, want_dw, first, last;
     int dz_rows;                // rows that dz has a place for: T rounded up to a K step of dW
+    int rest;                   // GRAD_RESTS: from this row on dz holds what rounding the rows before left
     int splits, split_steps;    // dX: K splits, 64-K steps of each
     int acc_groups;             // 32-row groups of acc, to the end of T
     float4 *acc;                // dX before its last sum: by split, 32 rows x 128 columns, 4 columns, lane
@@ -154,8 +162,8 @@ struct Units {
         steps_v = (a.d.vc + KB - 1) / KB;
         steps_n = (n + KB - 1) / KB;
         n_z = mt * nt_z;
-        n_dx = MODE == GRAD && a.want_dx && a.d.vc ? mt * nt_in * a.splits : 0;
-        n_dw = MODE == GRAD && a.want_dw ? mt_w * nt_in : 0;
+        n_dx = MODE != LOSS && a.want_dx && a.d.vc ? mt * nt_in * a.splits : 0;
+        n_dw = MODE != LOSS && a.want_dw ? mt_w * nt_in : 0;
         total = n_dx + n_dw + n_z;
     }
     // groups of row tiles; inside a group the rows run fastest, so the units in flight share
@@ -173,7 +181,7 @@ struct Units {
         int m = 0, c = 0;
         u.split = 0;
         u.step0 = 0;
-        if (MODE == GRAD && i < n_dx) {
+        if (MODE != LOSS && i < n_dx) {
             u.kind = DX;
             u.split = i / (mt * nt_in);
             place(i - u.split * (mt * nt_in), mt, nt_in, GROUP_D / TM, m, c);
@@ -373,6 +381,7 @@ __device__ __forceinline__ void loss_epilogue(const Args &a, float (&z)[HALF], R
             make_float2(m, ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])));
 }
 
+template <bool RESTS>
 __device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *out, uint32_t buf, float (&z)[HALF],
                                             RowTargets &tg, int t, int row0, int lane, bool live, int col0, float l2,
                                             float gt)
@@ -395,14 +404,26 @@ __device__ __forceinline__ void dz_epilogue(const Args &a, const CUtensorMap *ou
         for (int j = 0; j < HALF; j++) z[j] = 0.0f;
         gt = 0.0f;
     }
-    if (row0 >= a.dz_rows) return;         // (a multiple of 64: a warp's 32 rows lie on one side of it)
+    if (row0 >= (RESTS ? a.rest : a.dz_rows)) return;      // (multiples of 32: a warp's rows lie on one side)
+#pragma unroll 1
+    for (int part = 0;; part++) {
 #pragma unroll
-    for (int c0 = 0; c0 < HALF; c0 += 64)
-        store64(buf, out, col0 + c0, row0, false, lane, [&](int j) {
-            const float *f = z + c0 + 8 * j;
-            return make_uint4(pack_bf16(f[0] * gt, f[1] * gt), pack_bf16(f[2] * gt, f[3] * gt),
-                              pack_bf16(f[4] * gt, f[5] * gt), pack_bf16(f[6] * gt, f[7] * gt));
-        });
+        for (int c0 = 0; c0 < HALF; c0 += 64)
+            store64(buf, out, col0 + c0, RESTS ? row0 + part * a.rest : row0, false, lane, [&](int j) {
+                const float *f = z + c0 + 8 * j;
+                return make_uint4(pack_bf16(f[0] * gt, f[1] * gt), pack_bf16(f[2] * gt, f[3] * gt),
+                                  pack_bf16(f[4] * gt, f[5] * gt), pack_bf16(f[6] * gt, f[7] * gt));
+            });
+        if (!RESTS || part == 1) break;
+        if constexpr (RESTS) {
+#pragma unroll
+            for (int j = 0; j < HALF; j++) {
+                const float v = z[j] * gt, r = __bfloat162float(__float2bfloat16_rn(v));
+                z[j] = fabsf(r) < INFINITY ? v - r : 0.0f; // exact; nothing beside an infinity or a NaN
+            }
+            gt = 1.0f;
+        }
+    }
 }
 
 // dz was formed without these: exactly common factors add no rounding of their own to it
@@ -470,14 +491,15 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_release();
-    const int n_live = *a.n_live;
+    const int n_live = *a.n_live, n_rows = MODE == GRAD_RESTS && n_live ? a.rest + n_live : n_live;
     bool failed = false;
 
     if (warp == 0) {
         if (lane == 0) {
             const bool in_place = a.x_in_place && n_live == a.T;
             const CUtensorMap *xk = in_place ? &maps.x_k : &maps.xp_k, *xmn = in_place ? &maps.x_mn : &maps.xp_mn;
-            const Units<MODE, CG> units(a, n_live);
+            if (MODE == GRAD_RESTS) xmn = &maps.xp_mn;             // (its rows twice)
+            const Units<MODE, CG> units(a, n_rows);
             int item = 0, n_units = 0;
             for (int i = blockIdx.x / CG; !failed; i += gridDim.x / CG) {
                 const int slot = n_units % NU;
@@ -528,7 +550,7 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 bar_arrive(s_addr(&b_took[slot]));
                 if (t.kind < 0) break;
                 // A and B are K-major for z; dX takes W as rows of K, dW both operands so
-                const bool b_mn = MODE == GRAD && t.kind != Z, a_mn = MODE == GRAD && t.kind == DW;
+                const bool b_mn = MODE != LOSS && t.kind != Z, a_mn = MODE != LOSS && t.kind == DW;
                 const uint32_t idesc = (bf16_idesc(BN, b_mn) + ((uint32_t)(CG - 1) << 27)) | (a_mn ? (1u << 15) : 0u);
                 const uint32_t da = a_mn ? 2048u >> 4 : 32u >> 4, db = b_mn ? 2048u >> 4 : 32u >> 4;
                 const int chunk = b_mn ? t.steps : a.chunk;
@@ -628,8 +650,8 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                 if (MODE == LOSS) take(words_next, r_next);
                 if (MODE == LOSS) loss_epilogue(a, z, tg, r.x, row, live, col0);
                 else
-                    dz_epilogue(a, &maps.z_out, buf, z, tg, r.x, row0, lane, live, col0, __int_as_float(r.z),
-                                __int_as_float(r.w));
+                    dz_epilogue<MODE == GRAD_RESTS>(a, &maps.z_out, buf, z, tg, r.x, row0, lane, live, col0,
+                                                    __int_as_float(r.z), __int_as_float(r.w));
                 __syncwarp();
                 if (MODE != LOSS) take(words_next, r_next);
             } else if (t.kind == DW) {
@@ -657,11 +679,11 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
                     });
                 }
             } else {
-                const bool live = row < n_live;
+                const bool live = row < n_live || (MODE == GRAD_RESTS && row >= a.rest && row < n_rows);
                 const float scale = out_scale(a);
-                const bool sum = a.splits > 1 || !a.last, add = !a.first;
+                const bool sum = MODE == GRAD_RESTS || a.splits > 1 || !a.last, add = !a.first;
                 float4 *acc = a.acc + acc_at(a, t.split, row0, col0) + lane;
-                __nv_bfloat16 *out = live ? a.dX + (size_t)r.x * a.lddx : nullptr;
+                __nv_bfloat16 *out = row < n_live ? a.dX + (size_t)r.x * a.lddx : nullptr;
                 take(words_next, r_next);
                 if (t.steps > 0 && !finished()) { failed = true; break; }
                 for (int c0 = 0; c0 < HALF; c0 += 32) {
@@ -715,8 +737,8 @@ __global__ void __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant_
     }
 }
 
-// dX = the splits' sums in order, as bf16. Block (tile, p): columns 8 p .. and 128 + 8 p .. of a
-// 128 x 256 tile, a warp for 32 rows of each half.
+// dX = the splits' sums in order, each with its row's rest, as bf16. Block (tile, p): columns 8 p ..
+// and 128 + 8 p .. of a 128 x 256 tile, a warp for 32 rows of each half.
 __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
 {
     const int cols = (a.in + BN - 1) / BN, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -728,12 +750,21 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const Args a)
     if (row >= *a.n_live || col >= a.in) return;
     float4 f0 = make_float4(0, 0, 0, 0), f1 = f0;
     const float4 *p = a.acc + acc_at(a, 0, group, half) + (int)blockIdx.y * 64 + lane;
-    const size_t step = acc_at(a, 1, 0, 0);
-#pragma unroll 4
-    for (int s = 0; s < a.splits; s++, p += step) {
-        const float4 p0 = p[0], p1 = p[32];
+    const size_t step = acc_at(a, 1, 0, 0), rest = acc_at(a, 0, a.rest, 0);
+    auto add = [&](const float4 *q) {
+        const float4 p0 = q[0], p1 = q[32];
         f0.x += p0.x; f0.y += p0.y; f0.z += p0.z; f0.w += p0.w;
         f1.x += p1.x; f1.y += p1.y; f1.z += p1.z; f1.w += p1.w;
+    };
+    if (rest) {
+#pragma unroll 4
+        for (int s = 0; s < a.splits; s++, p += step) {
+            add(p);
+            add(p + rest);
+        }
+    } else {
+#pragma unroll 4
+        for (int s = 0; s < a.splits; s++, p += step) add(p);
     }
     put8(a.dX + (size_t)a.rows[row].x * a.lddx + col, f0, f1, out_scale(a), a.vec_dx);
 }
@@ -828,7 +859,8 @@ __global__ void __launch_bounds__(32 * TEACHER_ROWS) teacher_kernel(int *s_ids, 
 // counts the live ones before them itself (T * 4 bytes from L2, at most PACK_BLOCKS blocks),
 // so one launch does it. When every row counts and X can be read in place nothing is copied;
 // else the rows from the last packed one to the end of its K step become zeros: dW sums over
-// them. (What z's tiles read past those is of rows that do not count.)
+// them. (What z's tiles read past those is of rows that do not count.) With `rest` all of it stands
+// there a second time: what dW takes with the rests of dz.
 // The weights are divided by the mantissa of the largest of them (*g_scale): a mean's common
 // 1 / n is then a power of two, which rounds nothing when dz becomes bf16, and weights of
 // any ratio keep their range. (Where the largest is 0 or not finite, by 1.)
@@ -843,6 +875,7 @@ struct Pack {
     const uint16_t *X;
     const int *label, *count;          // one of them
     int lddx, ldx, vec, in_place;      // vec: X's rows lie on 16 bytes
+    int rest;                          // the packed rows stand at this row again (0: once)
     int T, in, vocab, per;
 };
 
@@ -907,7 +940,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
         *k.g_scale = g_scale;
     }
     __syncthreads();
-    const bool copy = !(k.in_place && total == T);
+    const bool copy = k.rest || !(k.in_place && total == T);
     // a warp takes a row's next PACK_COLS columns
     const int parts = (in + PACK_COLS - 1) / PACK_COLS;
     for (int w = warp; w < (t1 - t0) * parts; w += 8) {
@@ -915,15 +948,24 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
         if (p >= 0 && copy) {
             const uint16_t *x = k.X + (size_t)t * k.ldx;
             uint16_t *o = k.xp + (size_t)p * in;
+            const size_t again = (size_t)k.rest * in;
             if (k.vec) {
 #pragma unroll
                 for (int i = 0; i < PACK_COLS / 256; i++) {
                     const int c = c0 + (i * 32 + lane) * 8;
-                    if (c < c1) *reinterpret_cast<uint4 *>(o + c) = *reinterpret_cast<const uint4 *>(x + c);
+                    if (c < c1) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(x + c);
+                        *reinterpret_cast<uint4 *>(o + c) = v;
+                        if (again) *reinterpret_cast<uint4 *>(o + again + c) = v;
+                    }
                 }
             } else {
 #pragma unroll 8
-                for (int c = c0 + lane; c < c1; c += 32) o[c] = x[c];
+                for (int c = c0 + lane; c < c1; c += 32) {
+                    const uint16_t v = x[c];
+                    o[c] = v;
+                    if (again) o[again + c] = v;
+                }
             }
         }
         if (p < 0) {
@@ -935,10 +977,14 @@ __global__ void __launch_bounds__(256) pack_kernel(const Pack k)
                 for (int c = c0 + lane; c < c1; c += 32) k.dX[(size_t)t * k.lddx + c] = __float2bfloat16_rn(0.0f);
         }
     }
-    if (copy)
-        for (int p = total + (int)blockIdx.x * 8 + warp; p < (total + KB - 1) / KB * KB; p += (int)gridDim.x * 8)
-            for (int i = lane; i < in / 8; i += 32)
+    if (copy) {
+        const int end = k.rest ? k.rest : (total + KB - 1) / KB * KB;
+        for (int p = total + (int)blockIdx.x * 8 + warp; p < end; p += (int)gridDim.x * 8)
+            for (int i = lane; i < in / 8; i += 32) {
                 reinterpret_cast<uint4 *>(k.xp + (size_t)p * in)[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (k.rest) reinterpret_cast<uint4 *>(k.xp + (size_t)(k.rest + p) * in)[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+    }
 }
 
 // 32 packed rows a block, 32 threads a row: the tile halves' statistics joined in double.
@@ -1052,7 +1098,7 @@ static size_t a256(size_t b) { return (b + 255) & ~(size_t)255; }
 struct Plan {
     int cg;                            // CTAs that share a unit of the backward
     int Tpad, tiles, piece, pieces;    // vocabulary tiles; ids per piece of the backward; pieces
-    int dz_rows, acc_groups;           // rows of dz, 32-row groups of dX's sums
+    int rest, dz_rows, acc_groups;     // where dz's rests begin (0: none), its rows, 32-row groups of dX's sums
     int splits, split_steps;           // of dX's K (a piece)
     size_t dz_bytes, acc_bytes;        // of one piece; of dX's sums in fp32
 };
@@ -1087,16 +1133,17 @@ static Plan plan(int T, int in, int vocab)
     const long long tiles = std::max<long long>(8, (128LL << 20) / ((long long)p.Tpad * 2 * BN));
     p.piece = (int)std::min<long long>(tiles, p.tiles) * BN;
     p.pieces = ceil_div(vocab, p.piece);
-    p.dz_rows = ceil_div(T, KB) * KB;
+    p.rest = T <= 32 ? 32 : 0;
+    p.dz_rows = p.rest ? 2 * p.rest : ceil_div(T, KB) * KB;
     p.dz_bytes = (size_t)p.dz_rows * p.piece * 2;
     // dX has few tiles with long sums over the ids: split them where that shortens the busiest
     // worker of the launches, each unit's fp32 sums costing about 16 steps to write
     // and read back; the sums of all splits take 256 MB at most (a limit that only hidden states
-    // wider than 19,000 reach)
+    // wider than 16,384 reach)
     const int rows = ceil_div(T, BM * p.cg), cols = ceil_div(in, BN), steps = p.piece / KB;
     const int workers = PLAN_SMS / p.cg;
     const long long n_w = (long long)ceil_div(p.piece, BM * p.cg) * cols, n_z = (long long)rows * (p.piece / BN);
-    p.acc_groups = ceil_div(T, 32);
+    p.acc_groups = p.rest ? 2 * p.rest / 32 : ceil_div(T, 32);
     const size_t sums = (size_t)p.acc_groups * 32 * cols * BN * 4;
     double best = 0.0;
     p.splits = 1;
@@ -1114,7 +1161,7 @@ static Plan plan(int T, int in, int vocab)
     }
     p.split_steps = ceil_div(steps, p.splits);
     p.splits = ceil_div(steps, p.split_steps);
-    p.acc_bytes = p.pieces > 1 || p.splits > 1 ? p.splits * sums : 0;
+    p.acc_bytes = p.pieces > 1 || p.splits > 1 || p.rest ? p.splits * sums : 0;
     return p;
 }
 
@@ -1174,7 +1221,7 @@ static int prepare_device(int *sms)
     const uint64_t bit = 1ull << (dev & 63);
     if (dev < 64 && (ready.load() & bit)) return K3GPU_OK;
     for (const void *f : {(const void *)head_kernel<LOSS, 1>, (const void *)head_kernel<GRAD, 1>,
-                          (const void *)head_kernel<GRAD, 2>})
+                          (const void *)head_kernel<GRAD, 2>, (const void *)head_kernel<GRAD_RESTS, 1>})
         if ((st = cuda_status(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)))) return st;
     if (dev < 64) ready.fetch_or(bit);
     return K3GPU_OK;
@@ -1274,10 +1321,11 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
     Maps maps{};
     Pack k{};
     k.dX = reinterpret_cast<__nv_bfloat16 *>(dX); k.lddx = lddx; k.lse = lse; k.g = g;
+    k.rest = p.rest;
     if ((st = set_up(&a, &maps, c, p, w, k, p.cg, true))) return st;
     a.g_scale = g ? w.g_scale : nullptr;
     a.acc = w.acc;
-    a.dz_rows = p.dz_rows; a.acc_groups = p.acc_groups;
+    a.dz_rows = p.dz_rows; a.rest = p.rest; a.acc_groups = p.acc_groups;
     a.splits = p.splits; a.split_steps = p.split_steps;
     a.dX = reinterpret_cast<__nv_bfloat16 *>(dX);
     a.want_dx = dX != nullptr; a.want_dw = dW != nullptr;
@@ -1294,10 +1342,12 @@ static int backward(uint16_t *dX, int lddx, uint16_t *dW, const float *g, const 
             if ((st = map2d(&maps.dz_k, a.d.dz, a.d.vc, p.piece, p.dz_rows, BM))) return st;
             if ((st = map2d(&maps.dz_mn, a.d.dz, a.d.vc, p.piece, p.dz_rows, 64))) return st;
         }
-        st = p.cg == 1 ? launch_head<GRAD, 1>(maps, a, sms, c.s) : launch_head<GRAD, 2>(maps, a, sms, c.s);
+        st = p.rest      ? launch_head<GRAD_RESTS, 1>(maps, a, sms, c.s)
+             : p.cg == 1 ? launch_head<GRAD, 1>(maps, a, sms, c.s)
+                         : launch_head<GRAD, 2>(maps, a, sms, c.s);
         if (st) return st;
     }
-    if (dX && p.splits > 1) {
+    if (dX && (p.splits > 1 || p.rest)) {
         return launch_pdl(sum_splits_kernel, dim3(ceil_div(c.T, BM) * ceil_div(c.in, BN), HALF / 8), 256, 0, c.s, 1, a);
     }
     return K3GPU_OK;

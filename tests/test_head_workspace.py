@@ -39,11 +39,11 @@ def grad_bytes(T, n, V, K):
     """That copy; dz, bf16, of one piece of the vocabulary that holds all of it, else of two of 128 MB
     (of eight tiles of 256 ids, if that is more), its rows padded to 64; dX in fp32, its rows padded
     to 32, split 32 times at most and while the splits fit 256 MB together, unless one alone is
-    larger."""
+    larger; up to 32 rows two sets of them."""
     rows = up(T, 64)
     piece = max(8, 128 * MB // (up(T, 256) * 512)) * 256
     dz = rows * up(V, 256) * 2 if V <= piece else 2 * rows * piece * 2
-    one = up(T, 32) * up(n, 256) * 4
+    one = (64 if T <= 32 else up(T, 32)) * up(n, 256) * 4
     return up(T, 256) * n * 2 + dz + max(one, min(32 * one, 256 * MB)) + small(T, K) + GRAIN
 
 
@@ -64,7 +64,7 @@ def test_one_sweep_under_the_full_head(m):
     """9 rows over 163,840 ids, whose fp32 logits are 5.9 MB."""
     lib = m.lib
     assert lib.k3gpu_lm_head_xent_loss_workspace(9, 7168, 163840) < 7 * MB
-    assert lib.k3gpu_lm_head_xent_workspace(9, 7168, 163840) < 64 * MB
+    assert lib.k3gpu_lm_head_xent_workspace(9, 7168, 163840) < 70 * MB
 
 
 def test_a_loss_takes_its_own_size(m):
