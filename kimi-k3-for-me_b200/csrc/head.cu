@@ -30,8 +30,8 @@
 // rest of each rounding, as bf16, is a second set of rows, against W for dX (whose last sum joins
 // the two) and against a copy of X for dW; rows and rests together are one K step of it, the
 // products no more tiles than without. Loss and gradient of 4 rows of 1024 over 32,000 ids take 84
-// us against 80, of 32 rows of 7168 over 163,840 1.81 ms against 1.77. (Up to 64 rows it was two
-// K steps: 127 against 101 us at 64 rows of 1024, which are off by 0.0019 to 0.0024 without.)
+// us against 80, of 32 rows of 7168 over 163,840 1.81 ms against 1.77. (Up to 64 rows it would
+// be two K steps: 94 against 77 us at 64 rows of 1024, which are off by 0.0019 to 0.0024 without.)
 //
 // One persistent CTA per SM takes every n-th unit of work (10 warps):
 //   warp 0     TMA, a ring of 64-K stages: A 128 rows (16 KB), B 256 rows (32 KB)
@@ -47,11 +47,12 @@
 // without that 4.4e-6, and it costs 0.3% (the MMAs do not wait, two accumulators alternate;
 // every 512: 2.6e-7 and 1.5%). dX and dW end in bf16 and stay in TMEM.
 //
-// What bounds it: the tensor cores at the card's power limit. Alone, 2048 rows of 7168 over
-// 163,840 ids: the loss 3.12 ms (1.54 PFLOP/s, 0.91 of the measured burst rate), the gradient
-// 9.9 ms for the three products it runs (1.45), the tensor pipe 86-90% busy while the clock
-// falls to 1.34-1.46 GHz; back to back 14.8-15.1 ms together. A handful of rows is a weight
-// stream: 9 rows 0.39 ms, 6.0 TB/s of W.
+// What bounds it: the tensor cores, and the power limit that holds their clock down. One call after
+// a pause, 2048 rows of 7168 over 163,840 ids: the loss 3.2 ms (1.48 PFLOP/s, 0.87 of the measured
+// burst rate), the gradient 9.8 ms for the three products it runs (1.47), the tensor pipe 87-90%
+// busy while the clock falls to 1.34-1.45 GHz; back to back 14.8-15.2 ms together, 1.28 PFLOP/s of
+// the four products, where a library product sustains 1.41. A handful of rows is a weight stream:
+// 9 rows 372 us of kernel (6.3 TB/s of W), 417-428 us a pass.
 // Units dealt out by a counter instead of in turn cost 2-3% (neighbouring SMs then no longer
 // read the same W tile together), pairs in the forward 3%.
 // Every wait is bounded (a wait that gives up has waited seconds, longer than any copy in
