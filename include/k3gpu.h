@@ -420,9 +420,8 @@ int k3gpu_topk_logits(int *idx, float *val, const float *logits, int rows, int v
  * and dX's sums in fp32. dz (rows padded to 64) is whole where 256-padded rows of it take up to 128
  * MB, else two pieces of up to 128 MB (of 2048 ids above 32,768 rows). The sums (rows padded to 32,
  * up to 32 rows two sets) are split up to 32 times, within 256 MB, or one dX in fp32 where that is
- * larger. For few rows dz and the sums are larger than the logits. Of
- * 7168 columns over 163,840 ids: 9 rows 6.6 MB for the loss and 69 MB for both, 2048 rows 51 and
- * 416 MB.
+ * larger. For few rows dz and the sums are larger than the logits. Of 7168 columns over 163,840
+ * ids: 9 rows 6.6 MB for the loss and 69 MB for both, 2048 rows 51 and 416 MB.
  *
  * Softmax cross entropy: lse[t] = ln sum_v e^z[t][v], loss[t] = lse[t] - z[t][label[t]], fp32
  * [T]. A negative label is a row without a target: its loss, lse and gradient are 0, and
@@ -437,9 +436,9 @@ int k3gpu_lm_head_xent(float *loss, float *lse, const uint16_t *X, int ldx, cons
  *   dz[t][v] = g[t] (e^(z[t][v] - lse[t]) - [v == label[t]]),  dX = dz W,  dW = dz^T X
  * with g [T] the loss's incoming gradient (NULL: 1). dX [T][in] (row stride lddx) and dW
  * [vocab][in] (16-byte aligned) are bf16 bits, written whole, not added to; either may be
- * NULL (a frozen head needs no dW). dz is rounded to bf16 once, which adds an
- * error of the size of the outputs' own rounding; of up to 32 rows the rest of that rounding is
- * kept as bf16 too and adds none. The sums are fp32. Neither output may overlap an input. */
+ * NULL (a frozen head needs no dW). dz is rounded to bf16 once, which adds an error of the size
+ * of the outputs' own rounding; of up to 32 rows the rest of that rounding is kept as bf16 too
+ * and adds none. The sums are fp32. Neither output may overlap an input. */
 int k3gpu_lm_head_xent_grad(uint16_t *dX, int lddx, uint16_t *dW, const float *g,
                             const float *lse, const uint16_t *X, int ldx, const uint16_t *W,
                             const int *label, int in, int vocab, int T, void *workspace,
